@@ -479,6 +479,100 @@ int sar_plan_rows(const sar_schedule* prework, const sar_schedule* main_schedule
                   const sar_tuning_t* tuning, int compute_units, int same_launch,
                   sar_plan_row* rows, int row_cap, int* nrows, sar_plan_ptr* ptrs, int ptr_cap, int* nptrs);
 
+/* ---- block operators -----------------------------------------------------------------------------------------
+ * What the ranks of an emulated group exchange inside a model's block, next to the gradients: the sum of their
+ * partial outputs with the norms, gate and residual around it, and the tokens that travel to their experts and back.
+ * No counterpart in the reference, whose only collective is AllReduce.  Common to all calls: `device` is the GPU the
+ * memory lies on and `stream` the caller's hipStream_t on it (NULL = the null stream); the call puts kernels on that
+ * stream and returns, allocates nothing, waits for nothing, and may be captured into a hipGraph.  All pointers are
+ * device memory unless said otherwise, aligned to their element size, as long as the sizes say, and rows follow each
+ * other without gaps.  No output may overlap an input or another output.  Workspaces belong to one call until the
+ * stream has passed it (two captured graphs that may run at once need one each).  Nothing is launched when an
+ * argument is refused (SAR_EINVAL).
+ *
+ * The tokens are rows of one array sharded over the ranks by rows: nothing here depends on where a shard ends. */
+
+#define SAR_MAX_EXPERTS 1024
+#define SAR_MAX_TOPK 64
+#define SAR_MAX_NORM_DIM 16384
+
+/* Sorts the (token, choice) slots by expert.  experts[tokens][topk] holds expert numbers of index_bytes (4 or 8)
+ * each; a number outside [0, num_experts) drops its slot.  The sort is stable: rows of an expert keep the order of
+ * their slots.  row_of_slot[tokens * topk]: the slot's row, -1 = dropped.  slot_of_row[tokens * topk]: the slot of
+ * each row, -1 behind the last one.  offsets[num_experts + 1]: first row of each expert, then the number of rows.
+ * tokens * topk must stay below 2^31.  workspace: sar_route_workspace() bytes (0 for few slots: may be NULL). */
+uint64_t sar_route_workspace(int64_t tokens, int topk, int num_experts);
+int sar_route(int device, void* stream, const void* experts, int index_bytes, int64_t tokens, int topk, int num_experts,
+              int32_t* row_of_slot, int32_t* slot_of_row, int32_t* offsets, void* workspace, uint64_t workspace_bytes);
+
+/* rows[row_of_slot[t][k]][:] = tokens[t][:], and zeros in the rows behind offsets[num_experts].  With weights
+ * (elements of weight_dtype, NULL = none) rows are weights[t][k] * tokens[t][:], rounded once.  rows has
+ * tokens * topk rows of `dim` elements of dtype.  The gradient of sar_combine without a gradient of its weights, and,
+ * without weights, the way to the experts. */
+int sar_dispatch(int device, void* stream, int dtype, const void* token_rows, int64_t tokens, int topk, int64_t dim,
+                 const int32_t* row_of_slot, const int32_t* offsets, int num_experts, const void* weights, int weight_dtype,
+                 void* rows);
+
+/* out[t][:] = sum over k of weights[t][k] * rows[row_of_slot[t][k]][:], in k order in 32 bits and rounded once; dropped
+ * slots count nothing, whatever their weight.  weights NULL = all one (the gradient of sar_dispatch). */
+int sar_combine(int device, void* stream, int dtype, const void* rows, int64_t tokens, int topk, int64_t dim,
+                const int32_t* row_of_slot, const void* weights, int weight_dtype, void* out);
+
+/* Gradients of sar_combine with weights for grad[tokens][dim]: grad_rows as sar_dispatch of grad with the weights, and
+ * grad_weights[t][k] = <grad[t], rows[row_of_slot[t][k]]> in weight_dtype (0 for a dropped slot).  grad_rows may be
+ * NULL (not wanted). */
+int sar_combine_backward(int device, void* stream, int dtype, const void* grad, const void* rows, int64_t tokens, int topk,
+                         int64_t dim, const int32_t* row_of_slot, const int32_t* offsets, int num_experts,
+                         const void* weights, int weight_dtype, void* grad_rows, void* grad_weights);
+
+enum { SAR_GATE_NONE = 0, SAR_GATE_CHANNEL = 1, SAR_GATE_TOKEN = 2, SAR_GATE_FULL = 3 };
+
+/* y = sum of the partials in rank order;  u = y * rsqrt(mean(y^2) + eps) * post_weight  (u = y without post_weight);
+ * hidden = residual_scale * residual + gate * u;  normed = hidden * rsqrt(mean(hidden^2) + eps) * pre_weight, in 32
+ * bits, `normed` from the unrounded hidden; means run over a token's `dim` elements. */
+typedef struct sar_reduce_norm_args {
+    int32_t dtype;            /* of partials, residual, hidden, normed                                              */
+    int32_t pre_dtype;        /* of pre_weight: dtype or SAR_F32                                                    */
+    int32_t post_dtype;       /* of post_weight: the same                                                           */
+    int32_t gate_dtype;       /* of gate: the same                                                                  */
+    int32_t gate_kind;        /* SAR_GATE_*: gate holds nothing, dim, tokens or tokens * dim elements               */
+    int32_t sources;          /* partials: 1 .. SAR_MAX_RANKS                                                       */
+    int32_t copies;           /* copies of normed, back to back (one for each rank that gets it): 1 .. SAR_MAX_RANKS */
+    int32_t reserved;         /* 0                                                                                  */
+    int64_t tokens, dim;      /* dim: 1 .. SAR_MAX_NORM_DIM                                                         */
+    float eps, residual_scale;
+    const void* const* partials;   /* host array of `sources` device pointers to tokens * dim elements (unused by the
+                                      backward pass)                                                                */
+    const void* residual;
+    const void* pre_weight;   /* NULL: no norm behind the sum, no normed                                            */
+    const void* post_weight;  /* NULL: no norm in front of the residual                                             */
+    const void* gate;
+    void* hidden;             /* may be NULL                                                                        */
+    void* normed;             /* copies * tokens * dim; NULL without pre_weight                                     */
+    float* total;             /* y in 32 bits for the backward pass, tokens * dim; may be NULL                      */
+    float* stats;             /* the two rsqrt factors for the backward pass, 2 * tokens; may be NULL               */
+} sar_reduce_norm_args;
+int sar_reduce_norm(int device, void* stream, const sar_reduce_norm_args* args);
+
+/* Gradients.  `forward` is the forward call's struct, of which dtypes, sizes, gate, weights, residual and stats are
+ * read.  Any output may be NULL (not wanted).  Column sums run in a fixed order: the same inputs give the same bits. */
+typedef struct sar_reduce_norm_grads {
+    const void* total;        /* y: what the forward call wrote (total_dtype SAR_F32), or with one source that partial */
+    int32_t total_dtype;
+    int32_t reserved;         /* 0                                                                                  */
+    const void* grad_hidden;  /* tokens * dim, or NULL = zero                                                       */
+    const void* grad_normed;  /* copies * tokens * dim, or NULL = zero                                              */
+    void* grad_partials;      /* sources * tokens * dim: every rank's own copy of the gradient of its partial       */
+    void* grad_residual;      /* tokens * dim                                                                       */
+    void* grad_pre_weight;    /* dim, in pre_dtype                                                                  */
+    void* grad_post_weight;   /* dim, in post_dtype                                                                 */
+    void* grad_gate;          /* as gate, in gate_dtype                                                             */
+    void* workspace;          /* sar_reduce_norm_workspace() bytes                                                  */
+    uint64_t workspace_bytes;
+} sar_reduce_norm_grads;
+uint64_t sar_reduce_norm_workspace(int64_t tokens, int64_t dim, int dtype);
+int sar_reduce_norm_backward(int device, void* stream, const sar_reduce_norm_args* forward, const sar_reduce_norm_grads* grads);
+
 #ifdef __cplusplus
 }
 #endif

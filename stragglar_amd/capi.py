@@ -92,6 +92,21 @@ class ProbeResult(ctypes.Structure):
         return self.bytes_moved / self.best_ms / 1e6
 
 
+class ReduceNormArgs(ctypes.Structure):
+    """sar_reduce_norm_args: pointers as plain integers (None = NULL)."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "pre_dtype", "post_dtype", "gate_dtype", "gate_kind", "sources", "copies", "reserved")]
+                + [("tokens", ctypes.c_int64), ("dim", ctypes.c_int64), ("eps", ctypes.c_float), ("residual_scale", ctypes.c_float),
+                   ("partials", ctypes.POINTER(ctypes.c_void_p))]
+                + [(n, ctypes.c_void_p) for n in ("residual", "pre_weight", "post_weight", "gate", "hidden", "normed", "total", "stats")])
+
+
+class ReduceNormGrads(ctypes.Structure):
+    """sar_reduce_norm_grads."""
+    _fields_ = [("total", ctypes.c_void_p), ("total_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)] + [
+        (n, ctypes.c_void_p) for n in ("grad_hidden", "grad_normed", "grad_partials", "grad_residual", "grad_pre_weight",
+                                       "grad_post_weight", "grad_gate", "workspace")] + [("workspace_bytes", ctypes.c_uint64)]
+
+
 class Tuning(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("block", "unroll", "order", "cache_policy", "reuse_rounds", "reverse_odd", "segments",
                                                  "executor", "col_wgs", "col_block", "col_forward", "col_slots", "col_light_sync", "col_latency_plan", "col_split", "col_fuse_prework", "col_elide_stores", "col_fuse_chains", "col_fuse_copies", "arena_spread", "col_prework", "col_depth_first", "col_vectors")]
@@ -121,6 +136,8 @@ EXPORTS = [
     "sar_launch_bytes", "sar_sleep_ticks", "sar_stats", "sar_plan", "sar_plan_rows", "sar_default_tuning",
     "sar_run_static", "sar_static_scratch_bytes", "sar_rank_pointer", "sar_probe_streams",
     "sar_spread_yardstick", "sar_spread_is_elsewhere", "sar_spread_pick", "sar_alloc_rows", "sar_free_rows",
+    "sar_route_workspace", "sar_route", "sar_dispatch", "sar_combine", "sar_combine_backward",
+    "sar_reduce_norm", "sar_reduce_norm_workspace", "sar_reduce_norm_backward",
 ]
 
 
@@ -134,7 +151,7 @@ class Library:
                 "%s is missing: build it with `make -C stragglar_amd/csrc` (there is no CPU fallback)" % path)
         self.path = path
         L = self.lib = ctypes.CDLL(path)
-        vp, c_int, u64, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_size_t
+        vp, c_int, u64, sz, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_size_t, ctypes.c_int64
         P = ctypes.POINTER
         sig = {
             "sar_version": (c_int, []),
@@ -184,6 +201,14 @@ class Library:
             "sar_spread_pick": (c_int, [ctypes.c_float, P(ctypes.c_float), c_int, P(c_int)]),
             "sar_alloc_rows": (c_int, [vp, c_int, u64, P(vp), P(c_int), P(c_int)]),
             "sar_free_rows": (c_int, [vp]),
+            "sar_route_workspace": (u64, [i64, c_int, c_int]),
+            "sar_route": (c_int, [c_int, vp, vp, c_int, i64, c_int, c_int, vp, vp, vp, vp, u64]),
+            "sar_dispatch": (c_int, [c_int, vp, c_int, vp, i64, c_int, i64, vp, vp, c_int, vp, c_int, vp]),
+            "sar_combine": (c_int, [c_int, vp, c_int, vp, i64, c_int, i64, vp, vp, c_int, vp]),
+            "sar_combine_backward": (c_int, [c_int, vp, c_int, vp, vp, i64, c_int, i64, vp, vp, c_int, vp, c_int, vp, vp]),
+            "sar_reduce_norm": (c_int, [c_int, vp, P(ReduceNormArgs)]),
+            "sar_reduce_norm_workspace": (u64, [i64, i64, c_int]),
+            "sar_reduce_norm_backward": (c_int, [c_int, vp, P(ReduceNormArgs), P(ReduceNormGrads)]),
         }
         assert sorted(sig) == sorted(EXPORTS)
         for name, (res, args) in sig.items():

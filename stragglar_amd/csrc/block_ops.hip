@@ -1,0 +1,1234 @@
+// Block operators of an emulated group: what its ranks exchange inside a model's block.
+//
+//   sar_route             slots (token, choice) sorted by expert, stable
+//   sar_dispatch          tokens to their rows in expert order (and the gradient of sar_combine's rows)
+//   sar_combine           a token's rows back as their weighted sum (and the gradient of sar_dispatch)
+//   sar_reduce_norm       sum over the ranks' partial outputs, norm, gate, residual, norm, a copy for every rank
+//
+// All of it is bound by HBM, so the kernels read every input once and keep what they need again in registers.  Rows
+// are moved as 16-byte vectors whatever their alignment: gfx950 takes 16-byte accesses at any element boundary, and a
+// row whose length is no whole number of vectors ends in a vector that overlaps the one before it (both lanes compute
+// and store the same bits; sums leave the doubled elements out).  Only rows shorter than one vector go element by
+// element.
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "errors.hpp"
+#include "sar.h"
+
+namespace sar {
+namespace {
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef u4 u4_any __attribute__((aligned(2)));   // 16 bytes at any element boundary
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+
+constexpr int kWave = 64;
+
+// ---- vectors of elements ------------------------------------------------------------------------------------
+// VE elements of a type: 16 bytes of them, or one where rows are shorter than that.
+template <int DT> struct ElemSize { static constexpr int value = DT == SAR_F32 ? 4 : 2; };
+template <int DT> constexpr int kVec = 16 / ElemSize<DT>::value;
+
+template <int DT, int VE> struct Raw { typedef u4 T; };
+template <> struct Raw<SAR_F32, 1> { typedef uint32_t T; };
+template <> struct Raw<SAR_F16, 1> { typedef uint16_t T; };
+template <> struct Raw<SAR_BF16, 1> { typedef uint16_t T; };
+
+template <int DT, int VE>
+__device__ __forceinline__ typename Raw<DT, VE>::T load(const char* base, uint32_t byte) {
+    if constexpr (VE == 1) {
+        typedef __attribute__((address_space(1))) const typename Raw<DT, VE>::T* P;
+        return *(P)(base + byte);
+    } else {
+        typedef __attribute__((address_space(1))) const u4_any* P;
+        return *(P)(base + byte);
+    }
+}
+template <int DT, int VE>
+__device__ __forceinline__ void store(char* base, uint32_t byte, typename Raw<DT, VE>::T v) {
+    if constexpr (VE == 1) {
+        typedef __attribute__((address_space(1))) typename Raw<DT, VE>::T* P;
+        *(P)(base + byte) = v;
+    } else {
+        typedef __attribute__((address_space(1))) u4_any* P;
+        *(P)(base + byte) = v;
+    }
+}
+
+__device__ __forceinline__ float widen(uint32_t bits, int dt) {   // one 16-bit element in the low half
+    if (dt == SAR_BF16) return __uint_as_float(bits << 16);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+}
+
+template <int DT, int VE>
+__device__ __forceinline__ void unpack(typename Raw<DT, VE>::T r, float* x) {
+    if constexpr (VE == 1) {
+        if constexpr (DT == SAR_F32) x[0] = __uint_as_float(r);
+        else x[0] = widen(r, DT);
+    } else if constexpr (DT == SAR_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(r[i]);
+    } else if constexpr (DT == SAR_BF16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(r[i] << 16);
+            x[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t bits = r[i];   // a value of its own: __builtin_bit_cast of a vector's element reads element 0
+            const h2 h = __builtin_bit_cast(h2, bits);
+            x[2 * i] = (float)h.x;
+            x[2 * i + 1] = (float)h.y;
+        }
+    }
+}
+
+// The one rounding of a result: to nearest, ties to even.
+template <int DT, int VE>
+__device__ __forceinline__ typename Raw<DT, VE>::T pack(const float* x) {
+    if constexpr (VE == 1) {
+        if constexpr (DT == SAR_F32) return __float_as_uint(x[0]);
+        else if constexpr (DT == SAR_F16) return __builtin_bit_cast(uint16_t, (_Float16)x[0]);
+        else return __builtin_bit_cast(uint16_t, (__bf16)x[0]);
+    } else {
+        u4 r;
+        if constexpr (DT == SAR_F32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f2 p;
+                p.x = x[2 * i];
+                p.y = x[2 * i + 1];
+                if constexpr (DT == SAR_BF16) r[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf2));
+                else r[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, h2));
+            }
+        }
+        return r;
+    }
+}
+
+// VE parameters (weights, gate) from element `elem` on, held in DT or in 32 bits.
+template <int DT, int VE>
+__device__ __forceinline__ void load_param(const char* p, bool f32, uint32_t elem, float* x) {
+    if (DT == SAR_F32 || f32) {
+        if constexpr (VE == 1) {
+            x[0] = __uint_as_float(load<SAR_F32, 1>(p, elem * 4u));
+        } else {
+#pragma unroll
+            for (int q = 0; q < VE / 4; ++q) unpack<SAR_F32, 4>(load<SAR_F32, 4>(p, elem * 4u + 16u * q), x + 4 * q);
+        }
+    } else {
+        unpack<DT, VE>(load<DT, VE>(p, elem * (uint32_t)ElemSize<DT>::value), x);
+    }
+}
+template <int DT>
+__device__ __forceinline__ float load_one(const char* p, bool f32, uint64_t elem) {
+    float x;
+    if (DT == SAR_F32 || f32) x = ((const float*)p)[elem];
+    else unpack<DT, 1>(load<DT, 1>(p + elem * (uint64_t)ElemSize<DT>::value, 0), &x);
+    return x;
+}
+template <int DT>
+__device__ __forceinline__ void store_one(char* p, bool f32, uint64_t elem, float x) {
+    if (DT == SAR_F32 || f32) ((float*)p)[elem] = x;
+    else store<DT, 1>(p + elem * (uint64_t)ElemSize<DT>::value, 0, pack<DT, 1>(&x));
+}
+
+// ---- sums over lanes ----------------------------------------------------------------------------------------
+// The sum over a wave, in every lane; always the same order (lanes to the right, then rows of 16, then halves).
+__device__ __forceinline__ float wave_sum(float x) {
+#define SAR_DPP_ADD(ctrl, rows) \
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl, rows, 0xf, false))
+    SAR_DPP_ADD(0x111, 0xf);   // from 1, 2, 4, 8 lanes to the left within a row of 16
+    SAR_DPP_ADD(0x112, 0xf);
+    SAR_DPP_ADD(0x114, 0xf);
+    SAR_DPP_ADD(0x118, 0xf);
+    SAR_DPP_ADD(0x142, 0xa);   // last lane of rows 0 and 2 to rows 1 and 3
+    SAR_DPP_ADD(0x143, 0xc);   // lane 31 to the upper half
+#undef SAR_DPP_ADD
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), kWave - 1));
+}
+
+// Sums over a workgroup, in every lane.  `turn` alternates between two halves of the scratch, so that one barrier a
+// sum is enough: a half is written again only after everybody has passed the barrier of the sum in between.
+struct BlockSum {
+    float* scratch;   // 2 * 2 * 16 floats of LDS
+    uint32_t turn, waves, wave, lane;
+    __device__ __forceinline__ void operator()(float& a, float& b) {
+        a = wave_sum(a);
+        b = wave_sum(b);
+        if (waves == 1) return;
+        float* s = scratch + 32u * (turn & 1u);
+        ++turn;
+        if (lane == 0) { s[wave] = a; s[16 + wave] = b; }
+        __syncthreads();
+        a = b = 0.f;
+        for (uint32_t w = 0; w < waves; ++w) { a += s[w]; b += s[16 + w]; }
+    }
+    __device__ __forceinline__ void operator()(float& a) {
+        a = wave_sum(a);
+        if (waves == 1) return;
+        float* s = scratch + 32u * (turn & 1u);
+        ++turn;
+        if (lane == 0) s[wave] = a;
+        __syncthreads();
+        a = 0.f;
+        for (uint32_t w = 0; w < waves; ++w) a += s[w];
+    }
+};
+
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+
+// ---- route --------------------------------------------------------------------------------------------------
+// A stable counting sort.  A wave takes strips of 64 consecutive slots; lanes with the same expert find each other by
+// one ballot per bit of the expert number, so a slot's place among its equals in the strip is a population count, and
+// the wave's running count of each expert sits in LDS.  Nothing depends on the order in which waves arrive.
+// Up to kRouteOne slots one workgroup does it all in one launch; above, one launch counts the slots of each expert in
+// every block of kRouteBlock slots, one turns the counts into first rows, and one places the slots.
+constexpr uint32_t kRouteThreads = 1024, kRouteWaves = kRouteThreads / kWave;
+constexpr uint32_t kRouteOneStrips = 8, kRouteStrips = 4;
+constexpr uint32_t kRouteOne = kRouteThreads * kRouteOneStrips, kRouteBlock = kRouteThreads * kRouteStrips;
+constexpr uint32_t kDropped = 0xffffffffu;
+
+template <typename I>
+__device__ __forceinline__ uint32_t slot_expert(const I* experts, uint32_t n, uint32_t slot, uint32_t num_experts) {
+    if (slot >= n) return kDropped;
+    const I id = experts[slot];
+    return id >= 0 && id < (I)num_experts ? (uint32_t)id : kDropped;
+}
+
+// counts[expert][block]
+template <typename I>
+__global__ __launch_bounds__(kRouteThreads) void route_count_kernel(const I* __restrict__ experts, uint32_t n, uint32_t num_experts,
+                                                                    uint32_t* __restrict__ counts, uint32_t blocks) {
+    __shared__ uint32_t hist[SAR_MAX_EXPERTS];
+    const uint32_t tid = threadIdx.x, block = blockIdx.x;
+    if (tid < num_experts) hist[tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t s = 0; s < kRouteStrips; ++s) {
+        const uint32_t key = slot_expert(experts, n, block * kRouteBlock + s * kRouteThreads + tid, num_experts);
+        if (key != kDropped) atomicAdd(&hist[key], 1u);
+    }
+    __syncthreads();
+    if (tid < num_experts) counts[(uint64_t)tid * blocks + block] = hist[tid];
+}
+
+// One wave per expert: counts[expert][block] becomes the number of its slots in earlier blocks, totals[expert] all.
+__global__ __launch_bounds__(kWave) void route_scan_kernel(uint32_t* __restrict__ counts, uint32_t* __restrict__ totals, uint32_t blocks) {
+    uint32_t* const mine = counts + (uint64_t)blockIdx.x * blocks;
+    const uint32_t lane = threadIdx.x;
+    uint32_t before = 0;
+    for (uint32_t b = 0; b < blocks; b += kWave) {
+        const uint32_t v = b + lane < blocks ? mine[b + lane] : 0u;
+        uint32_t sum = v;
+        for (uint32_t d = 1; d < kWave; d <<= 1) {
+            const uint32_t left = __shfl_up(sum, d, kWave);
+            if (lane >= d) sum += left;
+        }
+        if (b + lane < blocks) mine[b + lane] = before + sum - v;
+        before += __shfl(sum, kWave - 1, kWave);
+    }
+    if (lane == 0) totals[blockIdx.x] = before;
+}
+
+template <typename I, uint32_t STRIPS, bool MANY>
+__global__ __launch_bounds__(kRouteThreads) void route_place_kernel(const I* __restrict__ experts, uint32_t n, uint32_t num_experts,
+                                                                    uint32_t key_bits, const uint32_t* __restrict__ counts,
+                                                                    const uint32_t* __restrict__ totals, uint32_t blocks,
+                                                                    int32_t* __restrict__ row_of_slot, int32_t* __restrict__ slot_of_row,
+                                                                    int32_t* __restrict__ offsets) {
+    __shared__ uint16_t seen[kRouteWaves * SAR_MAX_EXPERTS];   // slots of an expert: this wave's so far, then earlier waves'
+    __shared__ uint32_t first[SAR_MAX_EXPERTS];
+    __shared__ uint32_t wave_total[kRouteWaves];
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wave = uniform(tid / kWave);
+    const uint32_t begin = blockIdx.x * (kRouteThreads * STRIPS);
+    uint16_t* const mine = seen + wave * num_experts;
+    for (uint32_t i = lane; i < num_experts; i += kWave) mine[i] = 0;
+
+    uint32_t key[STRIPS], place[STRIPS];
+#pragma unroll
+    for (uint32_t s = 0; s < STRIPS; ++s)
+        key[s] = slot_expert(experts, n, begin + (wave * STRIPS + s) * kWave + lane, num_experts);
+    const uint64_t below = (1ull << lane) - 1ull;
+#pragma unroll
+    for (uint32_t s = 0; s < STRIPS; ++s) {
+        const bool in = key[s] != kDropped;
+        uint64_t equal = __ballot(in);
+        for (uint32_t b = 0; b < key_bits; ++b) {
+            const uint64_t set = __ballot((key[s] >> b) & 1u);
+            equal &= (key[s] >> b) & 1u ? set : ~set;
+        }
+        const uint32_t rank = (uint32_t)__popcll(equal & below);
+        // one wave's LDS accesses are done in order: every lane has read before the first of its equals writes
+        const uint32_t earlier = in ? mine[key[s]] : 0u;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (in && rank == 0) mine[key[s]] = (uint16_t)(earlier + (uint32_t)__popcll(equal));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        place[s] = earlier + rank;
+    }
+    __syncthreads();
+
+    uint32_t sum = 0;                                            // this block's slots of expert `tid`
+    if (tid < num_experts) {
+        for (uint32_t w = 0; w < kRouteWaves; ++w) {
+            const uint32_t v = seen[w * num_experts + tid];
+            seen[w * num_experts + tid] = (uint16_t)sum;
+            sum += v;
+        }
+        if (MANY) sum = totals[tid];
+    }
+    uint32_t upto = sum;                                         // inclusive sum over the experts, wave by wave
+    for (uint32_t d = 1; d < kWave; d <<= 1) {
+        const uint32_t left = __shfl_up(upto, d, kWave);
+        if (lane >= d) upto += left;
+    }
+    if (lane == kWave - 1) wave_total[wave] = upto;
+    __syncthreads();
+    uint32_t total = 0;
+    for (uint32_t w = 0; w < kRouteWaves; ++w) {
+        if (w < wave) upto += wave_total[w];
+        total += wave_total[w];
+    }
+    if (tid < num_experts) {
+        first[tid] = upto - sum + (MANY ? counts[(uint64_t)tid * blocks + blockIdx.x] : 0u);
+        if (blockIdx.x == 0) offsets[tid] = (int32_t)(upto - sum);
+    }
+    if (blockIdx.x == 0 && tid == 0) offsets[num_experts] = (int32_t)total;
+    __syncthreads();
+
+#pragma unroll
+    for (uint32_t s = 0; s < STRIPS; ++s) {
+        const uint32_t slot = begin + (wave * STRIPS + s) * kWave + lane;
+        if (slot >= n) continue;
+        const bool in = key[s] != kDropped;
+        const uint32_t row = in ? first[key[s]] + seen[wave * num_experts + key[s]] + place[s] : kDropped;
+        row_of_slot[slot] = (int32_t)row;
+        if (in) slot_of_row[row] = (int32_t)slot;
+        if (slot >= total) slot_of_row[slot] = -1;               // the rows behind the last one
+    }
+}
+
+// ---- dispatch, combine --------------------------------------------------------------------------------------
+// A wave takes one token (and a segment of 64 * U vectors of its row).  Lane k holds the row and the weight of choice k;
+// the choices that were not dropped are the bits of a ballot, walked in order with the row number in a scalar register.
+// Row numbers come from memory and are held against the number of rows before they become an address.
+constexpr uint32_t kMoveThreads = 256, kMoveWaves = kMoveThreads / kWave;
+
+struct MoveArgs {
+    const char* in;          // dispatch: tokens; combine: rows; backward: grad
+    const char* rows;        // backward: rows
+    char* out;               // dispatch: rows; combine: tokens; backward: grad_rows (may be null)
+    const char* weights;     // null: all one
+    char* grad_weights;
+    const int32_t* row_of_slot;
+    const int32_t* total;    // number of rows in use
+    uint64_t tokens;
+    uint32_t topk, nrows, dim, nvec, row_bytes, weights_f32;
+};
+
+// Zeros in the rows nobody was sent to: row total + token, and every `tokens`-th behind it.
+template <int DT, int VE, int U>
+__device__ __forceinline__ void zero_rows(const MoveArgs& a, uint64_t token, uint32_t v0) {
+    uint32_t total = uniform((uint32_t)*a.total);
+    if (total > a.nrows) total = a.nrows;
+    for (uint64_t row = total + token; row < a.nrows; row += a.tokens) {
+        char* const to = a.out + row * a.row_bytes;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t v = v0 + u * kWave;
+            if (v < a.nvec) store<DT, VE>(to, min(v * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value, typename Raw<DT, VE>::T{});
+        }
+    }
+}
+
+template <int DT, int VE, int U, bool WEIGHTED>
+__global__ __launch_bounds__(kMoveThreads) void dispatch_kernel(const MoveArgs a) {
+    typedef typename Raw<DT, VE>::T R;
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
+    const uint32_t v0 = blockIdx.x * (U * kWave) + lane;
+    for (uint64_t token = (uint64_t)blockIdx.y * kMoveWaves + wave; token < a.tokens; token += (uint64_t)gridDim.y * kMoveWaves) {
+        const uint64_t slot = token * a.topk + lane;
+        const uint32_t row = lane < a.topk ? (uint32_t)a.row_of_slot[slot] : kDropped;
+        float weight = 1.f;
+        if (WEIGHTED && lane < a.topk) weight = load_one<DT>(a.weights, a.weights_f32, slot);
+        const char* const from = a.in + token * a.row_bytes;
+        R v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (v0 + u * kWave < a.nvec) v[u] = load<DT, VE>(from, min((v0 + u * kWave) * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value);
+        for (uint64_t left = __ballot(row < a.nrows); left; left &= left - 1) {
+            const int k = __builtin_ctzll(left);
+            char* const to = a.out + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)row, k) * a.row_bytes;
+            const float w = WEIGHTED ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), k)) : 1.f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (v0 + u * kWave >= a.nvec) continue;
+                R r = v[u];
+                if constexpr (WEIGHTED) {
+                    float x[VE];
+                    unpack<DT, VE>(r, x);
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) x[i] *= w;
+                    r = pack<DT, VE>(x);
+                }
+                store<DT, VE>(to, min((v0 + u * kWave) * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value, r);
+            }
+        }
+        zero_rows<DT, VE, U>(a, token, v0);
+    }
+}
+
+// The sum is kept in 32 bits and taken in the order of the choices; four rows are loaded at a time.
+template <int DT, int VE, int U>
+__global__ __launch_bounds__(kMoveThreads) void combine_kernel(const MoveArgs a) {
+    typedef typename Raw<DT, VE>::T R;
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
+    const uint32_t v0 = blockIdx.x * (U * kWave) + lane;
+    for (uint64_t token = (uint64_t)blockIdx.y * kMoveWaves + wave; token < a.tokens; token += (uint64_t)gridDim.y * kMoveWaves) {
+        const uint64_t slot = token * a.topk + lane;
+        const uint32_t row = lane < a.topk ? (uint32_t)a.row_of_slot[slot] : kDropped;
+        float weight = 1.f;
+        if (a.weights && lane < a.topk) weight = load_one<DT>(a.weights, a.weights_f32, slot);
+        float sum[U][VE] = {};
+        uint64_t left = __ballot(row < a.nrows);
+        auto take = [&](auto count) {
+            constexpr int C = decltype(count)::value;
+            R v[C][U];
+            float w[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int k = __builtin_ctzll(left);
+                left &= left - 1;
+                const char* const from = a.in + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)row, k) * a.row_bytes;
+                w[c] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), k));
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (v0 + u * kWave < a.nvec) v[c][u] = load<DT, VE>(from, min((v0 + u * kWave) * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value);
+            }
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (v0 + u * kWave >= a.nvec) continue;
+                    float x[VE];
+                    unpack<DT, VE>(v[c][u], x);
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) sum[u][i] = fmaf(w[c], x[i], sum[u][i]);
+                }
+            }
+        };
+        int count = __popcll(left);
+        for (; count >= 4; count -= 4) take(std::integral_constant<int, 4>{});
+        if (count >= 2) { take(std::integral_constant<int, 2>{}); count -= 2; }
+        if (count) take(std::integral_constant<int, 1>{});
+        char* const to = a.out + token * a.row_bytes;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (v0 + u * kWave < a.nvec) store<DT, VE>(to, min((v0 + u * kWave) * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value, pack<DT, VE>(sum[u]));
+    }
+}
+
+// Both gradients in one pass over the rows: a token's gradient row stays in registers while its rows go by, each read
+// once for its dot product (summed in 32 bits, kept in the lane of its choice) and written once.  SHARE waves take one
+// token's segments in turn where the rows are long; their dot products are added in wave order.
+template <int DT, int VE, int U, int SHARE>
+__global__ __launch_bounds__(kMoveThreads) void combine_backward_kernel(const MoveArgs a) {
+    typedef typename Raw<DT, VE>::T R;
+    __shared__ float dots[kMoveWaves][kWave];
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
+    const uint32_t part = wave % SHARE;
+    constexpr uint32_t kTokens = kMoveWaves / SHARE;            // tokens a workgroup has in hand
+    for (uint64_t base = (uint64_t)blockIdx.x * kTokens; base < a.tokens; base += (uint64_t)gridDim.x * kTokens) {
+        const uint64_t token = base + wave / SHARE;
+        if (SHARE > 1 || token < a.tokens) {
+            const uint64_t slot = token * a.topk + lane;
+            const uint32_t row = lane < a.topk ? (uint32_t)a.row_of_slot[slot] : kDropped;
+            const float weight = lane < a.topk ? load_one<DT>(a.weights, a.weights_f32, slot) : 0.f;
+            const uint64_t present = __ballot(row < a.nrows);
+            const char* const grad = a.in + token * a.row_bytes;
+            float dot = 0.f;                                     // of choice `lane`
+            for (uint32_t seg = part * (U * kWave); seg < a.nvec; seg += SHARE * U * kWave) {
+                const uint32_t v0 = seg + lane;
+                R g[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (v0 + u * kWave < a.nvec) g[u] = load<DT, VE>(grad, min((v0 + u * kWave) * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value);
+                for (uint64_t left = present; left; left &= left - 1) {
+                    const int k = __builtin_ctzll(left);
+                    const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)row, k) * a.row_bytes;
+                    const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), k));
+                    R v[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (v0 + u * kWave < a.nvec) v[u] = load<DT, VE>(a.rows + at, min((v0 + u * kWave) * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value);
+                    float s = 0.f;
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const uint32_t vec = v0 + u * kWave;
+                        if (vec >= a.nvec) continue;
+                        const uint32_t e0 = min(vec * VE, a.dim - VE), twice = vec * VE - e0;
+                        float x[VE], y[VE];
+                        unpack<DT, VE>(g[u], x);
+                        unpack<DT, VE>(v[u], y);
+#pragma unroll
+                        for (int i = 0; i < VE; ++i) {
+                            s = (uint32_t)i >= twice ? fmaf(x[i], y[i], s) : s;
+                            x[i] *= w;
+                        }
+                        if (a.out) store<DT, VE>(a.out + at, e0 * (uint32_t)ElemSize<DT>::value, pack<DT, VE>(x));
+                    }
+                    s = wave_sum(s);
+                    if ((int)lane == k) dot += s;
+                }
+                if (a.out) zero_rows<DT, VE, U>(a, token, v0);
+            }
+            if (SHARE > 1) dots[wave][lane] = dot;
+            else if (lane < a.topk) store_one<DT>(a.grad_weights, a.weights_f32, slot, dot);
+        }
+        if (SHARE > 1) {
+            __syncthreads();
+            if (part == 0 && lane < a.topk) {
+                float dot = 0.f;
+                for (uint32_t p = 0; p < SHARE; ++p) dot += dots[wave + p][lane];
+                store_one<DT>(a.grad_weights, a.weights_f32, token * a.topk + lane, dot);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// ---- sum over the ranks, norms, gate, residual ----------------------------------------------------------------
+// A workgroup takes one token; its row stays in registers in 32 bits from the sum over the ranks to the last norm.
+struct NormArgs {
+    const char* partials[SAR_MAX_RANKS];
+    const char* residual;
+    const char* pre;
+    const char* post;
+    const char* gate;
+    char* hidden;
+    char* normed;
+    float* total;
+    float* stats;
+    uint64_t tokens, copy_bytes;
+    uint32_t dim, nvec, row_bytes, sources, copies, gate_kind, pre_f32, post_f32, gate_f32;
+    float eps, residual_scale, inv_dim;
+};
+
+constexpr uint32_t kNormThreads = 1024;
+
+template <int DT, int VE, int V>
+__global__ __launch_bounds__(kNormThreads) void reduce_norm_kernel(const NormArgs a) {
+    typedef typename Raw<DT, VE>::T R;
+    constexpr uint32_t ES = ElemSize<DT>::value;
+    __shared__ float scratch[64];
+    BlockSum sum{scratch, 0u, blockDim.x / kWave, uniform(threadIdx.x / kWave), threadIdx.x & (kWave - 1)};
+    for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
+        const uint64_t at = token * a.row_bytes;
+        float x[V][VE];
+        R res[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const uint32_t vec = threadIdx.x + v * blockDim.x;
+#pragma unroll
+            for (int i = 0; i < VE; ++i) x[v][i] = 0.f;
+            if (vec >= a.nvec) continue;
+            const uint32_t b = min(vec * VE, a.dim - VE) * ES;
+            res[v] = load<DT, VE>(a.residual + at, b);
+            unpack<DT, VE>(load<DT, VE>(a.partials[0] + at, b), x[v]);
+            uint32_t s = 1;
+            for (; s + 4 <= a.sources; s += 4) {
+                R p[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) p[q] = load<DT, VE>(a.partials[s + q] + at, b);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float y[VE];
+                    unpack<DT, VE>(p[q], y);
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) x[v][i] += y[i];
+                }
+            }
+            for (; s < a.sources; ++s) {
+                float y[VE];
+                unpack<DT, VE>(load<DT, VE>(a.partials[s] + at, b), y);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) x[v][i] += y[i];
+            }
+            if (a.total) {
+                char* const t = (char*)a.total + token * a.dim * 4u;
+                if constexpr (VE == 1) store<SAR_F32, 1>(t, b / ES * 4u, __float_as_uint(x[v][0]));
+                else {
+#pragma unroll
+                    for (int q = 0; q < VE / 4; ++q) store<SAR_F32, 4>(t, b / ES * 4u + 16u * q, pack<SAR_F32, 4>(x[v] + 4 * q));
+                }
+            }
+        }
+        float r1 = 1.f;
+        if (a.post) {
+            float ss = 0.f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const uint32_t vec = threadIdx.x + v * blockDim.x;
+                const uint32_t twice = vec < a.nvec ? vec * VE - min(vec * VE, a.dim - VE) : 0u;
+#pragma unroll
+                for (int i = 0; i < VE; ++i) ss = (uint32_t)i >= twice ? fmaf(x[v][i], x[v][i], ss) : ss;
+            }
+            sum(ss);
+            r1 = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
+        }
+        const float token_gate = a.gate_kind == SAR_GATE_TOKEN ? load_one<DT>(a.gate, a.gate_f32, token) : 1.f;
+        float ss = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const uint32_t vec = threadIdx.x + v * blockDim.x;
+            if (vec >= a.nvec) continue;
+            const uint32_t e0 = min(vec * VE, a.dim - VE), twice = vec * VE - e0;
+            float h[VE], w[VE];
+            unpack<DT, VE>(res[v], h);
+            if (a.post) {
+                load_param<DT, VE>(a.post, a.post_f32, e0, w);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) x[v][i] = x[v][i] * r1 * w[i];
+            }
+            if (a.gate_kind == SAR_GATE_CHANNEL || a.gate_kind == SAR_GATE_FULL) {
+                const uint64_t skip = a.gate_kind == SAR_GATE_FULL ? token * a.dim * (a.gate_f32 ? 4u : ES) : 0u;
+                load_param<DT, VE>(a.gate + skip, a.gate_f32, e0, w);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) w[i] = token_gate;
+            }
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                x[v][i] = fmaf(a.residual_scale, h[i], w[i] * x[v][i]);
+                ss = (uint32_t)i >= twice ? fmaf(x[v][i], x[v][i], ss) : ss;
+            }
+            if (a.hidden) store<DT, VE>(a.hidden + at, e0 * ES, pack<DT, VE>(x[v]));
+        }
+        float r2 = 1.f;
+        if (a.pre) {
+            sum(ss);
+            r2 = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const uint32_t vec = threadIdx.x + v * blockDim.x;
+                if (vec >= a.nvec) continue;
+                const uint32_t e0 = min(vec * VE, a.dim - VE);
+                float w[VE];
+                load_param<DT, VE>(a.pre, a.pre_f32, e0, w);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) x[v][i] = x[v][i] * r2 * w[i];
+                const R r = pack<DT, VE>(x[v]);
+                char* to = a.normed + at;
+                for (uint32_t c = 0; c < a.copies; ++c, to += a.copy_bytes) store<DT, VE>(to, e0 * ES, r);
+            }
+        }
+        if (a.stats && threadIdx.x == 0) { a.stats[token] = r1; a.stats[a.tokens + token] = r2; }
+    }
+}
+
+// With yhat = y r1, u = yhat post, hidden = s residual + g u, hhat = hidden r2, G = sum of the copies' gradients:
+//   d hidden   = grad_hidden + r2 (G pre - hhat mean(G pre hhat))      d residual = s d hidden       d pre  = sum_t G hhat
+//   d u        = g d hidden                                            d g = d hidden u, summed      d post = sum_t du yhat
+//   d partials = r1 (du post - yhat mean(du post yhat))
+// hidden is computed again from y and the residual, so nothing that was rounded comes back.  A workgroup walks over
+// tokens and keeps the column sums in registers; they leave as one row of sums per workgroup, added up by
+// column_sum_kernel in a fixed order.
+struct NormBackwardArgs {
+    NormArgs f;
+    const char* total;
+    const char* grad_hidden;
+    const char* grad_normed;
+    char* grad_partials;
+    char* grad_residual;
+    char* grad_gate;                   // per token or full (a channel gate's gradient is a column sum)
+    float* columns;                    // [workgroup][3][dim]
+    uint32_t total_f32, want_pre, want_post, want_gate;   // want_gate: a channel gate's
+};
+
+template <int DT, int VE, int V>
+__global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(const NormBackwardArgs b) {
+    typedef typename Raw<DT, VE>::T R;
+    constexpr uint32_t ES = ElemSize<DT>::value;
+    __shared__ float scratch[64];
+    const NormArgs& a = b.f;
+    BlockSum sum{scratch, 0u, blockDim.x / kWave, uniform(threadIdx.x / kWave), threadIdx.x & (kWave - 1)};
+    float col_pre[V][VE] = {}, col_post[V][VE] = {}, col_gate[V][VE] = {};
+    for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
+        const uint64_t at = token * a.row_bytes;
+        const float r1 = a.stats[token], r2 = a.stats[a.tokens + token];
+        const float token_gate = a.gate_kind == SAR_GATE_TOKEN ? load_one<DT>(a.gate, a.gate_f32, token) : 1.f;
+        float y[V][VE];      // yhat (y without a norm there)
+        float h[V][VE];      // hhat
+        float d[V][VE];      // G pre, then d hidden
+        float mean = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const uint32_t vec = threadIdx.x + v * blockDim.x;
+#pragma unroll
+            for (int i = 0; i < VE; ++i) y[v][i] = h[v][i] = d[v][i] = 0.f;
+            if (vec >= a.nvec) continue;
+            const uint32_t e0 = min(vec * VE, a.dim - VE), twice = vec * VE - e0;
+            load_param<DT, VE>(b.total + token * a.dim * (b.total_f32 ? 4u : ES), b.total_f32, e0, y[v]);
+            unpack<DT, VE>(load<DT, VE>(a.residual + at, e0 * ES), h[v]);
+            if (b.grad_normed) {
+                const char* from = b.grad_normed + at;
+                uint32_t c = 0;
+                for (; c + 4 <= a.copies; c += 4, from += 4 * a.copy_bytes) {
+                    R p[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) p[q] = load<DT, VE>(from + q * a.copy_bytes, e0 * ES);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float x[VE];
+                        unpack<DT, VE>(p[q], x);
+#pragma unroll
+                        for (int i = 0; i < VE; ++i) d[v][i] += x[i];
+                    }
+                }
+                for (; c < a.copies; ++c, from += a.copy_bytes) {
+                    float x[VE];
+                    unpack<DT, VE>(load<DT, VE>(from, e0 * ES), x);
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) d[v][i] += x[i];
+                }
+            }
+            float w[VE], g[VE];
+#pragma unroll
+            for (int i = 0; i < VE; ++i) { w[i] = 1.f; g[i] = token_gate; y[v][i] *= r1; }
+            if (a.post) load_param<DT, VE>(a.post, a.post_f32, e0, w);
+            if (a.gate_kind == SAR_GATE_CHANNEL) load_param<DT, VE>(a.gate, a.gate_f32, e0, g);
+            if (a.gate_kind == SAR_GATE_FULL) load_param<DT, VE>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, e0, g);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) h[v][i] = fmaf(a.residual_scale, h[v][i], g[i] * (y[v][i] * w[i])) * r2;
+            if (b.grad_normed) {
+                load_param<DT, VE>(a.pre, a.pre_f32, e0, w);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    col_pre[v][i] = fmaf(d[v][i], h[v][i], col_pre[v][i]);
+                    d[v][i] *= w[i];
+                    mean = (uint32_t)i >= twice ? fmaf(d[v][i], h[v][i], mean) : mean;
+                }
+            }
+        }
+        if (b.grad_normed) {
+            sum(mean);
+            mean *= a.inv_dim;
+        }
+        float dot = 0.f, gate_dot = 0.f;
+        float t[V][VE];      // du post
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const uint32_t vec = threadIdx.x + v * blockDim.x;
+            if (vec >= a.nvec) continue;
+            const uint32_t e0 = min(vec * VE, a.dim - VE), twice = vec * VE - e0;
+            if (b.grad_normed) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) d[v][i] = r2 * fmaf(-h[v][i], mean, d[v][i]);
+            }
+            float w[VE], g[VE], x[VE];
+            if (b.grad_hidden) {
+                unpack<DT, VE>(load<DT, VE>(b.grad_hidden + at, e0 * ES), x);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) d[v][i] += x[i];
+            }
+            if (b.grad_residual) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) x[i] = a.residual_scale * d[v][i];
+                store<DT, VE>(b.grad_residual + at, e0 * ES, pack<DT, VE>(x));
+            }
+#pragma unroll
+            for (int i = 0; i < VE; ++i) { w[i] = 1.f; g[i] = token_gate; }
+            if (a.post) load_param<DT, VE>(a.post, a.post_f32, e0, w);
+            if (a.gate_kind == SAR_GATE_CHANNEL) load_param<DT, VE>(a.gate, a.gate_f32, e0, g);
+            if (a.gate_kind == SAR_GATE_FULL) load_param<DT, VE>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, e0, g);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                const float du = d[v][i] * g[i];
+                x[i] = d[v][i] * (y[v][i] * w[i]);
+                col_gate[v][i] += x[i];
+                col_post[v][i] = fmaf(du, y[v][i], col_post[v][i]);
+                t[v][i] = du * w[i];
+                dot = (uint32_t)i >= twice ? fmaf(t[v][i], y[v][i], dot) : dot;
+                gate_dot += (uint32_t)i >= twice ? x[i] : 0.f;
+            }
+            if (a.gate_kind == SAR_GATE_FULL && b.grad_gate) {
+                char* const to = b.grad_gate + token * a.dim * (a.gate_f32 ? 4u : ES);
+                if (DT == SAR_F32 || a.gate_f32) {
+                    if constexpr (VE == 1) store<SAR_F32, 1>(to, e0 * 4u, __float_as_uint(x[0]));
+                    else {
+#pragma unroll
+                        for (int q = 0; q < VE / 4; ++q) store<SAR_F32, 4>(to, e0 * 4u + 16u * q, pack<SAR_F32, 4>(x + 4 * q));
+                    }
+                } else {
+                    store<DT, VE>(to, e0 * ES, pack<DT, VE>(x));
+                }
+            }
+        }
+        sum(dot, gate_dot);
+        if (a.gate_kind == SAR_GATE_TOKEN && b.grad_gate && threadIdx.x == 0) store_one<DT>(b.grad_gate, a.gate_f32, token, gate_dot);
+        if (b.grad_partials) {
+            dot *= a.inv_dim;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const uint32_t vec = threadIdx.x + v * blockDim.x;
+                if (vec >= a.nvec) continue;
+                const uint32_t e0 = min(vec * VE, a.dim - VE);
+                if (a.post) {
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) t[v][i] = r1 * fmaf(-y[v][i], dot, t[v][i]);
+                }
+                const R r = pack<DT, VE>(t[v]);
+                char* to = b.grad_partials + at;
+                for (uint32_t s = 0; s < a.sources; ++s, to += a.copy_bytes) store<DT, VE>(to, e0 * ES, r);
+            }
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const uint32_t vec = threadIdx.x + v * blockDim.x;
+        if (vec >= a.nvec) continue;
+        const uint32_t e0 = min(vec * VE, a.dim - VE);
+        float* const to = b.columns + (uint64_t)blockIdx.x * 3u * a.dim + e0;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+            if (b.want_pre) to[i] = col_pre[v][i];
+            if (b.want_post) to[a.dim + i] = col_post[v][i];
+            if (b.want_gate) to[2 * a.dim + i] = col_gate[v][i];
+        }
+    }
+}
+
+// Adds the workgroups' rows of column sums: 64 columns a workgroup, 16 waves taking every 16th row, then in wave order.
+struct ColumnArgs {
+    const float* columns;
+    char* out[3];
+    uint32_t f32[3];
+    uint32_t rows, dim;
+};
+template <int DT>
+__global__ __launch_bounds__(1024) void column_sum_kernel(const ColumnArgs a) {
+    __shared__ float part[16][kWave];
+    const uint32_t which = blockIdx.y, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    if (!a.out[which]) return;
+    const uint32_t col = blockIdx.x * kWave + lane;
+    float s = 0.f;
+    if (col < a.dim)
+        for (uint32_t r = wave; r < a.rows; r += 16) s += a.columns[((uint64_t)r * 3u + which) * a.dim + col];
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && col < a.dim) {
+        s = 0.f;
+        for (int w = 0; w < 16; ++w) s += part[w][lane];
+        store_one<DT>(a.out[which], a.f32[which], col, s);
+    }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------
+
+// Makes `device` current for a call and puts the caller's device back.
+class OnDevice {
+public:
+    explicit OnDevice(int device) {
+        err_ = hipGetDevice(&before_);
+        if (err_ == hipSuccess && before_ != device) { err_ = hipSetDevice(device); moved_ = err_ == hipSuccess; }
+    }
+    ~OnDevice() { if (moved_) (void)hipSetDevice(before_); }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+    hipError_t error() const { return err_; }
+private:
+    int before_ = 0;
+    bool moved_ = false;
+    hipError_t err_;
+};
+
+int refuse(const char* why) { return set_error(SAR_EINVAL, why); }
+int launched(const char* what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? (int)SAR_OK : set_error(SAR_EHIP, std::string(what) + ": " + hipGetErrorString(e));
+}
+int not_current(int device, hipError_t e) {
+    (void)hipGetLastError();
+    return set_error(e == hipErrorNoDevice || e == hipErrorInvalidDevice ? SAR_ENODEV : SAR_EHIP,
+                     "device " + std::to_string(device) + ": " + hipGetErrorString(e));
+}
+
+bool known_dtype(int dt) { return dt == SAR_F32 || dt == SAR_F16 || dt == SAR_BF16; }
+uint32_t elem_size(int dt) { return dt == SAR_F32 ? 4u : 2u; }
+bool aligned(const void* p, uint64_t to) { return (uintptr_t)p % to == 0; }
+
+// calls f(integral_constant<int, DT>) for the dtype
+template <class F> void with_dtype(int dt, F&& f) {
+    if (dt == SAR_F32) f(std::integral_constant<int, SAR_F32>{});
+    else if (dt == SAR_F16) f(std::integral_constant<int, SAR_F16>{});
+    else f(std::integral_constant<int, SAR_BF16>{});
+}
+
+uint64_t route_blocks(uint64_t n) { return (n + kRouteBlock - 1) / kRouteBlock; }
+
+template <typename I>
+void launch_route(hipStream_t st, const void* experts, uint32_t n, uint32_t num_experts, int32_t* row_of_slot, int32_t* slot_of_row,
+                  int32_t* offsets, uint32_t* workspace) {
+    const I* ids = (const I*)experts;
+    uint32_t bits = 0;
+    while ((1u << bits) < num_experts) ++bits;
+    if (n <= kRouteOne) {
+        route_place_kernel<I, kRouteOneStrips, false><<<1, kRouteThreads, 0, st>>>(ids, n, num_experts, bits, nullptr, nullptr, 1, row_of_slot, slot_of_row, offsets);
+        return;
+    }
+    const uint32_t blocks = (uint32_t)route_blocks(n);
+    uint32_t* const totals = workspace;
+    uint32_t* const counts = workspace + num_experts;
+    route_count_kernel<I><<<blocks, kRouteThreads, 0, st>>>(ids, n, num_experts, counts, blocks);
+    route_scan_kernel<<<num_experts, kWave, 0, st>>>(counts, totals, blocks);
+    route_place_kernel<I, kRouteStrips, true><<<blocks, kRouteThreads, 0, st>>>(ids, n, num_experts, bits, counts, totals, blocks, row_of_slot, slot_of_row, offsets);
+}
+
+// What dispatch, combine and its backward pass have in common; null pointers that a call does not use are its own affair.
+const char* check_move(int dtype, int64_t tokens, int topk, int64_t dim, const int32_t* row_of_slot, const void* weights, int weight_dtype) {
+    if (!known_dtype(dtype)) return "unknown dtype";
+    if (tokens < 0) return "tokens is negative";
+    if (topk < 1 || topk > SAR_MAX_TOPK) return "topk must be 1 to 64";
+    if (tokens > INT32_MAX / topk) return "tokens * topk must stay below 2^31";
+    if (dim < 1 || dim > (1 << 24)) return "dim must be 1 to 2^24";
+    if (weights && weight_dtype != SAR_F32 && weight_dtype != dtype) return "weights must be of dtype or 32-bit floats";
+    if (weights && !aligned(weights, elem_size(weight_dtype))) return "weights are not aligned to their element size";
+    if (tokens && (!row_of_slot || !aligned(row_of_slot, 4))) return "row_of_slot is null or not aligned";
+    return nullptr;
+}
+
+MoveArgs move_args(int dtype, int64_t tokens, int topk, int64_t dim, const int32_t* row_of_slot, const void* weights, int weight_dtype) {
+    MoveArgs a{};
+    a.weights = (const char*)weights;
+    a.row_of_slot = row_of_slot;
+    a.tokens = (uint64_t)tokens;
+    a.topk = (uint32_t)topk;
+    a.nrows = (uint32_t)(tokens * topk);
+    a.dim = (uint32_t)dim;
+    const uint32_t ve = (uint32_t)dim < 16u / elem_size(dtype) ? 1u : 16u / elem_size(dtype);
+    a.nvec = (a.dim + ve - 1) / ve;
+    a.row_bytes = a.dim * elem_size(dtype);
+    a.weights_f32 = weight_dtype == SAR_F32;
+    return a;
+}
+
+// Vectors per lane: four where that still leaves every CU its waves, one where there are few tokens (the smallest
+// calls are bound by the time of one trip to memory, and more waves make it one trip instead of four).
+int move_vectors(const MoveArgs& a) {
+    const uint64_t segments = (a.nvec + 4 * kWave - 1) / (4 * kWave);
+    return a.tokens * segments >= 4096 && a.nvec > kWave ? 4 : 1;
+}
+
+dim3 move_grid(const MoveArgs& a, int u) {
+    const uint64_t groups = (a.tokens + kMoveWaves - 1) / kMoveWaves;
+    return dim3((a.nvec + u * kWave - 1) / (u * kWave), (uint32_t)std::min<uint64_t>(groups, 65535u));
+}
+
+template <int DT> void launch_dispatch(hipStream_t st, const MoveArgs& a) {
+    const int u = move_vectors(a);
+    const dim3 grid = move_grid(a, u);
+    if (a.dim < kVec<DT>) {
+        if (a.weights) dispatch_kernel<DT, 1, 1, true><<<grid, kMoveThreads, 0, st>>>(a);
+        else dispatch_kernel<DT, 1, 1, false><<<grid, kMoveThreads, 0, st>>>(a);
+    } else if (u == 4) {
+        if (a.weights) dispatch_kernel<DT, kVec<DT>, 4, true><<<grid, kMoveThreads, 0, st>>>(a);
+        else dispatch_kernel<DT, kVec<DT>, 4, false><<<grid, kMoveThreads, 0, st>>>(a);
+    } else {
+        if (a.weights) dispatch_kernel<DT, kVec<DT>, 1, true><<<grid, kMoveThreads, 0, st>>>(a);
+        else dispatch_kernel<DT, kVec<DT>, 1, false><<<grid, kMoveThreads, 0, st>>>(a);
+    }
+}
+
+template <int DT> void launch_combine(hipStream_t st, const MoveArgs& a) {
+    const int u = move_vectors(a);
+    const dim3 grid = move_grid(a, u);
+    if (a.dim < kVec<DT>) combine_kernel<DT, 1, 1><<<grid, kMoveThreads, 0, st>>>(a);
+    else if (u == 4) combine_kernel<DT, kVec<DT>, 4><<<grid, kMoveThreads, 0, st>>>(a);
+    else combine_kernel<DT, kVec<DT>, 1><<<grid, kMoveThreads, 0, st>>>(a);
+}
+
+template <int DT> void launch_combine_backward(hipStream_t st, const MoveArgs& a) {
+    const bool shared = a.nvec > 4 * kWave;
+    const uint64_t groups = shared ? a.tokens : (a.tokens + kMoveWaves - 1) / kMoveWaves;
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(groups, 1u << 20);
+    if (a.dim < kVec<DT>) combine_backward_kernel<DT, 1, 1, 1><<<grid, kMoveThreads, 0, st>>>(a);
+    else if (shared) combine_backward_kernel<DT, kVec<DT>, 2, 4><<<grid, kMoveThreads, 0, st>>>(a);
+    else combine_backward_kernel<DT, kVec<DT>, 4, 1><<<grid, kMoveThreads, 0, st>>>(a);
+}
+
+// Threads and vectors per thread for a row: one vector a thread as far as 1024 threads reach.
+struct NormShape { uint32_t threads; int vectors; bool single; };
+NormShape norm_shape(int dtype, int64_t dim) {
+    const uint32_t ve = 16u / elem_size(dtype);
+    if ((uint32_t)dim < ve) return {kWave, 1, true};
+    const uint32_t nvec = ((uint32_t)dim + ve - 1) / ve;
+    const int v = nvec <= 1024 ? 1 : nvec <= 2048 ? 2 : 4;
+    const uint32_t threads = ((nvec + v - 1) / v + kWave - 1) / kWave * kWave;
+    return {threads, v, false};
+}
+
+// Workgroups of the backward pass: as many as the chip holds at once, with a few tokens for each so that the column
+// sums are a small part of the traffic.
+uint32_t norm_backward_groups(int64_t tokens, int64_t dim, int dtype) {
+    const uint32_t waves = norm_shape(dtype, dim).threads / kWave;
+    const uint64_t resident = 256u * std::max(1u, std::min(4u, 16u / waves));
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(resident, ((uint64_t)tokens + 3) / 4));
+}
+
+const char* check_norm(const sar_reduce_norm_args* a) {
+    if (!a) return "the argument struct is null";
+    if (!known_dtype(a->dtype)) return "unknown dtype";
+    if (a->tokens < 0) return "tokens is negative";
+    if (a->dim < 1 || a->dim > SAR_MAX_NORM_DIM) return "dim must be 1 to 16384";
+    if (a->tokens > (int64_t)1 << 40) return "too many tokens";
+    if (a->sources < 1 || a->sources > SAR_MAX_RANKS) return "sources must be 1 to 64";
+    if (a->copies < 1 || a->copies > SAR_MAX_RANKS) return "copies must be 1 to 64";
+    if (!(a->eps >= 0.f) || a->eps > 3.4e38f) return "eps must be a number, zero or more";
+    if (a->pre_weight && a->pre_dtype != a->dtype && a->pre_dtype != SAR_F32) return "pre_weight must be of dtype or 32-bit floats";
+    if (a->post_weight && a->post_dtype != a->dtype && a->post_dtype != SAR_F32) return "post_weight must be of dtype or 32-bit floats";
+    if (a->gate_kind < SAR_GATE_NONE || a->gate_kind > SAR_GATE_FULL) return "unknown gate kind";
+    if (a->gate_kind != SAR_GATE_NONE && !a->gate && a->tokens) return "gate is null";
+    if (a->gate_kind != SAR_GATE_NONE && a->gate_dtype != a->dtype && a->gate_dtype != SAR_F32) return "gate must be of dtype or 32-bit floats";
+    const uint64_t es = elem_size(a->dtype);
+    if (!aligned(a->residual, es) || !aligned(a->pre_weight, a->pre_weight ? elem_size(a->pre_dtype) : 1) ||
+        !aligned(a->post_weight, a->post_weight ? elem_size(a->post_dtype) : 1) || !aligned(a->gate, a->gate_kind ? elem_size(a->gate_dtype) : 1))
+        return "a pointer is not aligned to its element size";
+    if (a->tokens && !a->residual) return "residual is null";
+    return nullptr;
+}
+
+NormArgs norm_args(const sar_reduce_norm_args* a) {
+    NormArgs k{};
+    k.residual = (const char*)a->residual;
+    k.pre = (const char*)a->pre_weight;
+    k.post = (const char*)a->post_weight;
+    k.gate = (const char*)a->gate;
+    k.hidden = (char*)a->hidden;
+    k.normed = (char*)a->normed;
+    k.total = a->total;
+    k.stats = a->stats;
+    k.tokens = (uint64_t)a->tokens;
+    k.dim = (uint32_t)a->dim;
+    const uint32_t es = elem_size(a->dtype), ve = a->dim < 16 / es ? 1u : 16u / es;
+    k.nvec = (k.dim + ve - 1) / ve;
+    k.row_bytes = k.dim * es;
+    k.copy_bytes = k.tokens * k.row_bytes;
+    k.sources = (uint32_t)a->sources;
+    k.copies = (uint32_t)a->copies;
+    k.gate_kind = (uint32_t)a->gate_kind;
+    k.pre_f32 = a->pre_dtype == SAR_F32;
+    k.post_f32 = a->post_dtype == SAR_F32;
+    k.gate_f32 = a->gate_dtype == SAR_F32;
+    k.eps = a->eps;
+    k.residual_scale = a->residual_scale;
+    k.inv_dim = 1.f / (float)a->dim;
+    return k;
+}
+
+template <int DT> void launch_norm(hipStream_t st, const NormArgs& a, const NormShape& s) {
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(a.tokens, 1u << 20);
+    if (s.single) reduce_norm_kernel<DT, 1, 1><<<grid, s.threads, 0, st>>>(a);
+    else if (s.vectors == 1) reduce_norm_kernel<DT, kVec<DT>, 1><<<grid, s.threads, 0, st>>>(a);
+    else if (s.vectors == 2) reduce_norm_kernel<DT, kVec<DT>, 2><<<grid, s.threads, 0, st>>>(a);
+    else if constexpr (DT == SAR_F32) reduce_norm_kernel<DT, kVec<DT>, 4><<<grid, s.threads, 0, st>>>(a);
+}
+
+template <int DT> void launch_norm_backward(hipStream_t st, const NormBackwardArgs& a, const NormShape& s, uint32_t grid) {
+    if (s.single) reduce_norm_backward_kernel<DT, 1, 1><<<grid, s.threads, 0, st>>>(a);
+    else if (s.vectors == 1) reduce_norm_backward_kernel<DT, kVec<DT>, 1><<<grid, s.threads, 0, st>>>(a);
+    else if (s.vectors == 2) reduce_norm_backward_kernel<DT, kVec<DT>, 2><<<grid, s.threads, 0, st>>>(a);
+    else if constexpr (DT == SAR_F32) reduce_norm_backward_kernel<DT, kVec<DT>, 4><<<grid, s.threads, 0, st>>>(a);
+}
+
+}  // namespace
+}  // namespace sar
+
+using namespace sar;
+
+extern "C" {
+
+uint64_t sar_route_workspace(int64_t tokens, int topk, int num_experts) {
+    if (tokens < 0 || topk < 1 || topk > SAR_MAX_TOPK || num_experts < 1 || num_experts > SAR_MAX_EXPERTS || tokens > INT32_MAX / topk) return 0;
+    const uint64_t n = (uint64_t)tokens * (uint64_t)topk;
+    return n <= kRouteOne ? 0 : (route_blocks(n) + 1) * (uint64_t)num_experts * 4u;
+}
+
+int sar_route(int device, void* stream, const void* experts, int index_bytes, int64_t tokens, int topk, int num_experts,
+              int32_t* row_of_slot, int32_t* slot_of_row, int32_t* offsets, void* workspace, uint64_t workspace_bytes) {
+    return guarded([&]() -> int {
+        if (index_bytes != 4 && index_bytes != 8) return refuse("index_bytes must be 4 or 8");
+        if (tokens < 0) return refuse("tokens is negative");
+        if (topk < 1 || topk > SAR_MAX_TOPK) return refuse("topk must be 1 to 64");
+        if (num_experts < 1 || num_experts > SAR_MAX_EXPERTS) return refuse("num_experts must be 1 to 1024");
+        if (tokens > INT32_MAX / topk) return refuse("tokens * topk must stay below 2^31");
+        if (!offsets || !aligned(offsets, 4)) return refuse("offsets is null or not aligned");
+        if (tokens && (!experts || !row_of_slot || !slot_of_row)) return refuse("a pointer is null");
+        if (!aligned(experts, (uint64_t)index_bytes) || !aligned(row_of_slot, 4) || !aligned(slot_of_row, 4)) return refuse("a pointer is not aligned to its element size");
+        const uint64_t need = sar_route_workspace(tokens, topk, num_experts);
+        if (need && (!workspace || !aligned(workspace, 4) || workspace_bytes < need)) return refuse("the workspace is smaller than sar_route_workspace()");
+        OnDevice on(device);
+        if (on.error() != hipSuccess) return not_current(device, on.error());
+        const uint32_t n = (uint32_t)(tokens * topk);
+        if (index_bytes == 8) launch_route<int64_t>((hipStream_t)stream, experts, n, (uint32_t)num_experts, row_of_slot, slot_of_row, offsets, (uint32_t*)workspace);
+        else launch_route<int32_t>((hipStream_t)stream, experts, n, (uint32_t)num_experts, row_of_slot, slot_of_row, offsets, (uint32_t*)workspace);
+        return launched("sar_route");
+    });
+}
+
+int sar_dispatch(int device, void* stream, int dtype, const void* token_rows, int64_t tokens, int topk, int64_t dim,
+                 const int32_t* row_of_slot, const int32_t* offsets, int num_experts, const void* weights, int weight_dtype,
+                 void* rows) {
+    return guarded([&]() -> int {
+        if (const char* why = check_move(dtype, tokens, topk, dim, row_of_slot, weights, weight_dtype)) return refuse(why);
+        if (num_experts < 1 || num_experts > SAR_MAX_EXPERTS) return refuse("num_experts must be 1 to 1024");
+        if (tokens == 0) return SAR_OK;
+        if (!token_rows || !rows || !offsets) return refuse("a pointer is null");
+        if (!aligned(token_rows, elem_size(dtype)) || !aligned(rows, elem_size(dtype)) || !aligned(offsets, 4)) return refuse("a pointer is not aligned to its element size");
+        OnDevice on(device);
+        if (on.error() != hipSuccess) return not_current(device, on.error());
+        MoveArgs a = move_args(dtype, tokens, topk, dim, row_of_slot, weights, weight_dtype);
+        a.in = (const char*)token_rows;
+        a.out = (char*)rows;
+        a.total = offsets + num_experts;
+        with_dtype(dtype, [&](auto dt) { launch_dispatch<decltype(dt)::value>((hipStream_t)stream, a); });
+        return launched("sar_dispatch");
+    });
+}
+
+int sar_combine(int device, void* stream, int dtype, const void* rows, int64_t tokens, int topk, int64_t dim,
+                const int32_t* row_of_slot, const void* weights, int weight_dtype, void* out) {
+    return guarded([&]() -> int {
+        if (const char* why = check_move(dtype, tokens, topk, dim, row_of_slot, weights, weight_dtype)) return refuse(why);
+        if (tokens == 0) return SAR_OK;
+        if (!rows || !out) return refuse("a pointer is null");
+        if (!aligned(rows, elem_size(dtype)) || !aligned(out, elem_size(dtype))) return refuse("a pointer is not aligned to its element size");
+        OnDevice on(device);
+        if (on.error() != hipSuccess) return not_current(device, on.error());
+        MoveArgs a = move_args(dtype, tokens, topk, dim, row_of_slot, weights, weight_dtype);
+        a.in = (const char*)rows;
+        a.out = (char*)out;
+        with_dtype(dtype, [&](auto dt) { launch_combine<decltype(dt)::value>((hipStream_t)stream, a); });
+        return launched("sar_combine");
+    });
+}
+
+int sar_combine_backward(int device, void* stream, int dtype, const void* grad, const void* rows, int64_t tokens, int topk,
+                         int64_t dim, const int32_t* row_of_slot, const int32_t* offsets, int num_experts,
+                         const void* weights, int weight_dtype, void* grad_rows, void* grad_weights) {
+    return guarded([&]() -> int {
+        if (const char* why = check_move(dtype, tokens, topk, dim, row_of_slot, weights, weight_dtype)) return refuse(why);
+        if (num_experts < 1 || num_experts > SAR_MAX_EXPERTS) return refuse("num_experts must be 1 to 1024");
+        if (tokens == 0) return SAR_OK;
+        if (!grad || !rows || !weights || !grad_weights || (grad_rows && !offsets)) return refuse("a pointer is null");
+        const uint64_t es = elem_size(dtype);
+        if (!aligned(grad, es) || !aligned(rows, es) || !aligned(grad_rows, es) || !aligned(offsets, 4) || !aligned(grad_weights, elem_size(weight_dtype)))
+            return refuse("a pointer is not aligned to its element size");
+        OnDevice on(device);
+        if (on.error() != hipSuccess) return not_current(device, on.error());
+        MoveArgs a = move_args(dtype, tokens, topk, dim, row_of_slot, weights, weight_dtype);
+        a.in = (const char*)grad;
+        a.rows = (const char*)rows;
+        a.out = (char*)grad_rows;
+        a.grad_weights = (char*)grad_weights;
+        a.total = offsets + num_experts;
+        with_dtype(dtype, [&](auto dt) { launch_combine_backward<decltype(dt)::value>((hipStream_t)stream, a); });
+        return launched("sar_combine_backward");
+    });
+}
+
+int sar_reduce_norm(int device, void* stream, const sar_reduce_norm_args* args) {
+    return guarded([&]() -> int {
+        if (const char* why = check_norm(args)) return refuse(why);
+        if (args->tokens == 0) return SAR_OK;
+        if (!args->partials) return refuse("the list of partials is null");
+        const uint64_t es = elem_size(args->dtype);
+        for (int s = 0; s < args->sources; ++s)
+            if (!args->partials[s] || !aligned(args->partials[s], es)) return refuse("a partial is null or not aligned to its element size");
+        if ((args->pre_weight != nullptr) != (args->normed != nullptr)) return refuse("pre_weight and normed go together");
+        if (!aligned(args->hidden, es) || !aligned(args->normed, es) || !aligned(args->total, 4) || !aligned(args->stats, 4))
+            return refuse("a pointer is not aligned to its element size");
+        OnDevice on(device);
+        if (on.error() != hipSuccess) return not_current(device, on.error());
+        NormArgs a = norm_args(args);
+        for (int s = 0; s < args->sources; ++s) a.partials[s] = (const char*)args->partials[s];
+        const NormShape shape = norm_shape(args->dtype, args->dim);
+        with_dtype(args->dtype, [&](auto dt) { launch_norm<decltype(dt)::value>((hipStream_t)stream, a, shape); });
+        return launched("sar_reduce_norm");
+    });
+}
+
+uint64_t sar_reduce_norm_workspace(int64_t tokens, int64_t dim, int dtype) {
+    if (tokens < 0 || dim < 1 || dim > SAR_MAX_NORM_DIM || !known_dtype(dtype)) return 0;
+    return (uint64_t)norm_backward_groups(tokens, dim, dtype) * 3u * (uint64_t)dim * 4u;
+}
+
+int sar_reduce_norm_backward(int device, void* stream, const sar_reduce_norm_args* forward, const sar_reduce_norm_grads* g) {
+    return guarded([&]() -> int {
+        if (const char* why = check_norm(forward)) return refuse(why);
+        if (!g) return refuse("the struct of gradients is null");
+        const uint64_t es = elem_size(forward->dtype);
+        const bool channel = forward->gate_kind == SAR_GATE_CHANNEL;
+        if (g->grad_normed && !forward->pre_weight) return refuse("grad_normed without pre_weight");
+        if (g->grad_pre_weight && !forward->pre_weight) return refuse("grad_pre_weight without pre_weight");
+        if (g->grad_post_weight && !forward->post_weight) return refuse("grad_post_weight without post_weight");
+        if (g->grad_gate && forward->gate_kind == SAR_GATE_NONE) return refuse("grad_gate without a gate");
+        if (g->total_dtype != SAR_F32 && g->total_dtype != forward->dtype) return refuse("total must be of dtype or 32-bit floats");
+        if (forward->tokens && (!g->total || !forward->stats)) return refuse("total or stats is null");
+        if (!aligned(g->total, elem_size(g->total_dtype)) || !aligned(forward->stats, 4) || !aligned(g->grad_hidden, es) || !aligned(g->grad_normed, es) ||
+            !aligned(g->grad_partials, es) || !aligned(g->grad_residual, es) ||
+            !aligned(g->grad_pre_weight, g->grad_pre_weight ? elem_size(forward->pre_dtype) : 1) ||
+            !aligned(g->grad_post_weight, g->grad_post_weight ? elem_size(forward->post_dtype) : 1) ||
+            !aligned(g->grad_gate, g->grad_gate ? elem_size(forward->gate_dtype) : 1))
+            return refuse("a pointer is not aligned to its element size");
+        if (!g->workspace || !aligned(g->workspace, 4) || g->workspace_bytes < sar_reduce_norm_workspace(forward->tokens, forward->dim, forward->dtype))
+            return refuse("the workspace is smaller than sar_reduce_norm_workspace()");
+        OnDevice on(device);
+        if (on.error() != hipSuccess) return not_current(device, on.error());
+        NormBackwardArgs b{};
+        b.f = norm_args(forward);
+        b.total = (const char*)g->total;
+        b.total_f32 = g->total_dtype == SAR_F32;
+        b.grad_hidden = (const char*)g->grad_hidden;
+        b.grad_normed = (const char*)g->grad_normed;
+        b.grad_partials = (char*)g->grad_partials;
+        b.grad_residual = (char*)g->grad_residual;
+        b.grad_gate = channel ? nullptr : (char*)g->grad_gate;
+        b.columns = (float*)g->workspace;
+        b.want_pre = g->grad_pre_weight != nullptr;
+        b.want_post = g->grad_post_weight != nullptr;
+        b.want_gate = channel && g->grad_gate != nullptr;
+        const uint32_t groups = norm_backward_groups(forward->tokens, forward->dim, forward->dtype);
+        const NormShape shape = norm_shape(forward->dtype, forward->dim);
+        with_dtype(forward->dtype, [&](auto dt) { launch_norm_backward<decltype(dt)::value>((hipStream_t)stream, b, shape, groups); });
+        if (int rc = launched("sar_reduce_norm_backward")) return rc;
+        if (b.want_pre || b.want_post || b.want_gate) {
+            ColumnArgs c{};
+            c.columns = b.columns;
+            c.out[0] = (char*)g->grad_pre_weight;
+            c.out[1] = (char*)g->grad_post_weight;
+            c.out[2] = channel ? (char*)g->grad_gate : nullptr;
+            c.f32[0] = b.f.pre_f32;
+            c.f32[1] = b.f.post_f32;
+            c.f32[2] = b.f.gate_f32;
+            c.rows = groups;
+            c.dim = b.f.dim;
+            const dim3 grid((c.dim + kWave - 1) / kWave, 3);
+            with_dtype(forward->dtype, [&](auto dt) { column_sum_kernel<decltype(dt)::value><<<grid, 1024, 0, (hipStream_t)stream>>>(c); });
+            return launched("sar_reduce_norm_backward");
+        }
+        return SAR_OK;
+    });
+}
+
+}  // extern "C"

@@ -14,16 +14,20 @@
 #include <vector>
 
 #include "column_plan.hpp"
+#include "errors.hpp"
 #include "kernels.hpp"
 #include "placed_pool.hpp"
 #include "sar.h"
 #include "schedule.hpp"
 
+namespace { thread_local std::string g_error; }
+
+int sar::set_error(int code, const std::string& msg) { g_error = msg; return code; }
+
 namespace {
 
-thread_local std::string g_error;
-
-int set_error(int code, const std::string& msg) { g_error = msg; return code; }
+using sar::guarded;
+using sar::set_error;
 
 #define SAR_HIP(expr)                                                                                   \
     do {                                                                                                \
@@ -45,14 +49,6 @@ struct Launch {
 };
 
 int elem_size_of(int dtype) { return dtype == SAR_F32 ? 4 : 2; }
-
-// Runs the body of an entry point; no exception leaves the C ABI.
-template <class F> int guarded(F&& body) {
-    try { return body(); }
-    catch (const std::bad_alloc&) { return set_error(SAR_ENOMEM, "out of host memory"); }
-    catch (const std::exception& e) { return set_error(SAR_EINVAL, e.what()); }
-    catch (...) { return set_error(SAR_EINVAL, "unexpected error"); }
-}
 
 }  // namespace
 

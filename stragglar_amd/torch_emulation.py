@@ -25,7 +25,7 @@ from typing import List, Optional, Sequence
 # two runtimes and the one initialised second reports "no ROCm-capable device is detected".
 import torch  # noqa: F401
 
-from . import capi
+from . import block_ops, capi
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _TORCH_DTYPES = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16"}
@@ -233,3 +233,56 @@ class EmulatedGroup:
                 g.copy_(flat[off:off + g.numel()].view_as(g))
                 off += g.numel()
         return flats
+
+    # ---- inside a transformer block: block_ops.py --------------------------------------------------------------
+    # The rest of what the ranks of a model exchange.  A block's tokens are the rows of one tensor, sharded over the
+    # ranks by rows (where a shard ends does not matter); rank r owns experts [r * E / n, (r + 1) * E / n).  Tensors are
+    # contiguous, float32, float16 or bfloat16, on the group's device.  All calls are asynchronous on torch's current
+    # stream and differentiable; under torch.no_grad() they and the *_backward calls may be captured into a graph.
+
+    def route(self, experts, num_experts: int) -> "block_ops.Routing":
+        """Sorts the slots of ``experts`` [tokens, topk] (int32 or int64 expert numbers) by expert, stable: where
+        ``dispatch`` puts every copy of a token and ``combine`` finds it.  A number outside 0 .. num_experts - 1 drops
+        its slot; the same expert may be chosen twice.  At most 64 choices, 1024 experts (a multiple of the ranks)."""
+        return block_ops.route(self, experts, num_experts)
+
+    def dispatch(self, tokens, routing):
+        """The tokens [tokens, dim] on their way to the experts: [tokens * topk, dim] sorted by expert, zeros behind the
+        last row in use (``routing.offsets[-1]``).  Rank r receives rows ``rank_offsets[r]`` to ``rank_offsets[r + 1]``."""
+        return block_ops.dispatch(self, tokens, routing)
+
+    def combine(self, rows, routing, weights=None):
+        """The experts' outputs back at their tokens: the sum over a token's choices of ``weights`` [tokens, topk]
+        (float32 or the rows' dtype; None = all one) times its rows, in 32 bits and rounded once.  Dropped slots count
+        nothing.  Differentiable in rows and weights."""
+        return block_ops.combine(self, rows, routing, weights)
+
+    def dispatch_backward(self, grad, routing):
+        """The gradient of ``dispatch``'s tokens for a gradient of its rows."""
+        return block_ops.dispatch_backward(self, grad, routing)
+
+    def combine_backward(self, grad, rows, routing, weights=None):
+        """The gradients (rows, weights) of ``combine``; rows nobody was sent to get zeros, dropped slots a zero weight
+        gradient, and without weights the second is None."""
+        return block_ops.combine_backward(self, grad, rows, routing, weights)
+
+    def reduce_norm(self, partials, residual, pre_weight=None, post_weight=None, gate=None, residual_scale: float = 1.0,
+                    eps: float = 1e-6, gather: bool = True, save: bool = False):
+        """The boundary of a block in one call: the sum of the ranks' partial outputs, the norm behind the block
+        (``post_weight``), its gate, the scaled residual and the norm in front of the next block (``pre_weight``):
+
+            y = sum of the partials;  u = rms_norm(y) * post_weight;  hidden = residual_scale * residual + gate * u
+            normed = rms_norm(hidden) * pre_weight,  rms_norm(x) = x / sqrt(mean(x^2) + eps)
+
+        ``partials``: one tensor [tokens, dim] per rank, or the ranks' as one [n, tokens, dim], or a finished output
+        [tokens, dim] that needs no sum.  ``gate``: [dim], [tokens, 1] or [tokens, dim]; weights and gate may be float32
+        beside 16-bit tensors; without a weight that norm is left out.  All of it is computed in 32 bits and rounded
+        once.  Returns (hidden [tokens, dim], normed): with ``gather`` normed is [n, tokens, dim], every rank's own
+        copy, else [tokens, dim]; None without ``pre_weight``.  With ``save`` a third value for ``reduce_norm_backward``
+        (inputs must then stay as they are until it has run).  At most 16384 columns."""
+        return block_ops.reduce_norm(self, partials, residual, pre_weight, post_weight, gate, residual_scale, eps, gather, save)
+
+    def reduce_norm_backward(self, saved, grad_hidden=None, grad_normed=None) -> "block_ops.ReduceNormGrads":
+        """The gradients of ``reduce_norm`` (partials, residual, pre_weight, post_weight, gate) for gradients of its
+        outputs (None = zero)."""
+        return block_ops.reduce_norm_backward(self, saved, grad_hidden, grad_normed)

@@ -1,0 +1,179 @@
+"""Refusals of the block operators (routing, dispatch, combine, reduce_norm): none of them needs a device, every one is
+said before anything is launched."""
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from stragglar_amd import block_ops, capi  # noqa: E402
+from stragglar_amd.torch_emulation import EmulatedGroup  # noqa: E402
+
+
+@pytest.fixture()
+def group(sarlib):
+    """A group without a context: the argument checks run before the device is touched."""
+    g = object.__new__(EmulatedGroup)
+    g.n, g.device, g._lib = 4, 0, sarlib
+    return g
+
+
+def routing(tokens=3, topk=2, experts=8):
+    return block_ops.Routing(torch.zeros(tokens, topk, dtype=torch.int32), torch.zeros(tokens * topk, dtype=torch.int32),
+                             torch.zeros(experts + 1, dtype=torch.int32), experts, 4)
+
+
+def test_route_refuses(group):
+    ids = torch.zeros(3, 2, dtype=torch.int64)
+    for bad, experts, why in [(ids.float(), 8, "dtype"), (ids.view(-1), 8, "tokens, topk"), (ids, 7, "multiple"), (ids, 0, "multiple"),
+                              (ids, 1028, "multiple"), (torch.zeros(3, 0, dtype=torch.int64), 8, "topk"),
+                              (torch.zeros(1, 65, dtype=torch.int32), 8, "topk"), (ids.t(), 8, "contiguous"), (ids, 8, "CUDA"),
+                              ([[0]], 8, "tokens, topk"), (torch.zeros(1, 1, dtype=torch.int64).expand(1 << 30, 2), 8, "contiguous")]:
+        with pytest.raises((ValueError, TypeError), match=why):
+            group.route(bad, experts)
+
+
+def test_dispatch_and_combine_refuse(group):
+    r = routing()
+    for call, why in [(lambda: group.dispatch(torch.zeros(4, 8), r), "tokens must be"),
+                      (lambda: group.dispatch(torch.zeros(3, 8, dtype=torch.float64), r), "dtype"),
+                      (lambda: group.dispatch(torch.zeros(3, 0), r), "columns"),
+                      (lambda: group.dispatch(torch.zeros(8, 3).t(), r), "must be|contiguous"),
+                      (lambda: group.dispatch(torch.zeros(3, 8), (1, 2, 3)), "routing"),
+                      (lambda: group.dispatch(torch.zeros(3, 8), r), "CUDA"),
+                      (lambda: group.combine(torch.zeros(5, 8), r), "rows must be"),
+                      (lambda: group.combine(torch.zeros(6, 8), r, torch.zeros(2, 3)), "weights has shape"),
+                      (lambda: group.combine(torch.zeros(6, 8), r, torch.zeros(3, 2).half()), "weights has dtype"),
+                      (lambda: group.combine(torch.zeros(6, 8).bfloat16(), r, torch.zeros(3, 2).half()), "weights has dtype"),
+                      (lambda: group.combine(torch.zeros(6, 8), r, torch.zeros(2, 3).t()), "contiguous"),
+                      (lambda: group.combine(torch.zeros(6, 8), r, torch.zeros(3, 2)), "CUDA"),
+                      (lambda: group.dispatch_backward(torch.zeros(3, 8), r), "grad must be"),
+                      (lambda: group.combine_backward(torch.zeros(3, 7), torch.zeros(6, 8), r), "grad has shape"),
+                      (lambda: group.combine_backward(torch.zeros(3, 8).half(), torch.zeros(6, 8), r), "grad has dtype")]:
+        with pytest.raises((ValueError, TypeError), match=why):
+            call()
+
+
+def test_reduce_norm_refuses(group):
+    t, d = 3, 8
+    x, w = torch.zeros(t, d), torch.ones(d)
+    for call, why in [(lambda: group.reduce_norm([x] * 3, x, w), "per emulated rank"),
+                      (lambda: group.reduce_norm([x] * 3 + [x[:2]], x, w), "shape"),
+                      (lambda: group.reduce_norm([x] * 3 + [x.half()], x, w), "dtype"),
+                      (lambda: group.reduce_norm(torch.zeros(3, t, d), x, w), "partials must be"),
+                      (lambda: group.reduce_norm(torch.zeros(t, d + 1), x, w), "partials must be"),
+                      (lambda: group.reduce_norm(x, x.double(), w), "dtype"),
+                      (lambda: group.reduce_norm(x, x.view(-1), w), "residual must be"),
+                      (lambda: group.reduce_norm(x, x, w[:4]), "pre_weight has shape"),
+                      (lambda: group.reduce_norm(x, x, w.half()), "pre_weight has dtype"),
+                      (lambda: group.reduce_norm(x, x, w, post_weight=torch.ones(1, d)), "post_weight has shape"),
+                      (lambda: group.reduce_norm(x, x, w, gate=torch.ones(1, d)), "gate must be"),
+                      (lambda: group.reduce_norm(x, x, w, gate=torch.ones(t)), "gate must be"),
+                      (lambda: group.reduce_norm(x, x, w, gate=torch.ones(1, d).expand(t, d)), "contiguous"),
+                      (lambda: group.reduce_norm(x, x, w, eps=-1.0), "eps"),
+                      (lambda: group.reduce_norm(x, x, w, eps=float("nan")), "eps"),
+                      (lambda: group.reduce_norm(torch.zeros(1, 16385), torch.zeros(1, 16385)), "dim must be"),
+                      (lambda: group.reduce_norm(torch.zeros(1, 0), torch.zeros(1, 0)), "dim must be"),
+                      (lambda: group.reduce_norm(x, x, w), "CUDA")]:
+        with pytest.raises((ValueError, TypeError), match=why):
+            call()
+
+
+def test_reduce_norm_backward_refuses(group):
+    x = torch.zeros(3, 8)
+    saved = block_ops.ReduceNormSaved(1, 4, (3, 8), x, torch.zeros(2, 3), x, torch.ones(8), None, None, 1.0, 1e-6)
+    for call, why in [(lambda: group.reduce_norm_backward((1, 2)), "saved"),
+                      (lambda: group.reduce_norm_backward(saved, torch.zeros(3, 7)), "grad_hidden has shape"),
+                      (lambda: group.reduce_norm_backward(saved, None, torch.zeros(3, 8)), "grad_normed has shape"),
+                      (lambda: group.reduce_norm_backward(saved, None, torch.zeros(4, 3, 8).half()), "dtype"),
+                      (lambda: group.reduce_norm_backward(saved._replace(pre_weight=None), None, torch.zeros(4, 3, 8)), "without a pre_weight"),
+                      (lambda: group.reduce_norm_backward(saved, x, None), "CUDA")]:
+        with pytest.raises((ValueError, TypeError), match=why):
+            call()
+
+
+def refused(lib, rc, why):
+    assert rc == -1 and why in lib.lib.sar_last_error().decode(), (rc, lib.lib.sar_last_error())
+
+
+def test_c_entries_refuse(sarlib):
+    """The C entry points say SAR_EINVAL before they look for a device (addresses here are never used)."""
+    L, p, odd = sarlib.lib, 0x10000, 0x10001
+    big = 1 << 40
+    route = lambda **k: L.sar_route(0, None, *[{**dict(experts=p, ib=8, t=4, k=2, e=8, r=p, s=p, o=p, w=None, wb=0), **k}[n]
+                                               for n in ("experts", "ib", "t", "k", "e", "r", "s", "o", "w", "wb")])
+    for k, why in [(dict(ib=2), "index_bytes"), (dict(t=-1), "negative"), (dict(k=0), "topk"), (dict(k=65), "topk"), (dict(e=0), "num_experts"),
+                   (dict(e=1025), "num_experts"), (dict(t=1 << 30), "2^31"), (dict(o=None), "offsets"), (dict(experts=None), "null"),
+                   (dict(experts=p + 4), "aligned"), (dict(r=odd), "aligned"), (dict(t=8192), "workspace"),
+                   (dict(t=8192, w=p, wb=8), "workspace")]:
+        refused(sarlib, route(**k), why)
+    assert L.sar_route_workspace(16, 8, 64) == 0 and L.sar_route_workspace(8192, 2, 8) == (4 + 1) * 8 * 4 and L.sar_route_workspace(-1, 2, 8) == 0
+
+    dispatch = lambda **k: L.sar_dispatch(0, None, *[{**dict(dt=0, x=p, t=4, k=2, d=8, r=p, o=p, e=8, w=None, wd=0, out=p), **k}[n]
+                                                     for n in ("dt", "x", "t", "k", "d", "r", "o", "e", "w", "wd", "out")])
+    combine = lambda **k: L.sar_combine(0, None, *[{**dict(dt=0, x=p, t=4, k=2, d=8, r=p, w=None, wd=0, out=p), **k}[n]
+                                                   for n in ("dt", "x", "t", "k", "d", "r", "w", "wd", "out")])
+    back = lambda **k: L.sar_combine_backward(0, None, *[{**dict(dt=0, g=p, x=p, t=4, k=2, d=8, r=p, o=p, e=8, w=p, wd=0, gr=p, gw=p), **k}[n]
+                                                         for n in ("dt", "g", "x", "t", "k", "d", "r", "o", "e", "w", "wd", "gr", "gw")])
+    for call in (dispatch, combine, back):
+        for k, why in [(dict(dt=3), "dtype"), (dict(t=-1), "negative"), (dict(k=0), "topk"), (dict(k=65), "topk"), (dict(d=0), "dim"),
+                       (dict(d=big), "dim"), (dict(t=1 << 30), "2^31"), (dict(r=None), "row_of_slot"), (dict(r=odd), "row_of_slot"),
+                       (dict(w=p, wd=1), "weights"), (dict(w=odd, wd=0), "weights"), (dict(x=None), "null"), (dict(x=odd), "aligned")]:
+            refused(sarlib, call(**k), why)
+        assert call(t=0) == 0
+    for call in (dispatch, combine):
+        refused(sarlib, call(out=None), "null")
+    refused(sarlib, dispatch(e=0), "num_experts")
+    refused(sarlib, dispatch(o=None), "null")
+    for k in (dict(g=None), dict(w=None), dict(gw=None), dict(o=None)):
+        refused(sarlib, back(**k), "null")
+
+    def norm(backward=False, grads=None, **k):
+        a = capi.ReduceNormArgs(dtype=0, sources=1, copies=1, tokens=4, dim=8, eps=1e-6, residual_scale=1.0, residual=p, hidden=p)
+        a.partials = (ctypes.c_void_p * 1)(p)
+        for n, v in k.items():
+            setattr(a, n, v)
+        if not backward:
+            return L.sar_reduce_norm(0, None, ctypes.byref(a))
+        g = capi.ReduceNormGrads(total=p, grad_hidden=p, grad_partials=p, workspace=p, workspace_bytes=1 << 30)
+        for n, v in (grads or {}).items():
+            setattr(g, n, v)
+        a.stats = k.get("stats", p)
+        return L.sar_reduce_norm_backward(0, None, ctypes.byref(a), ctypes.byref(g))
+
+    both = [(dict(dtype=3), "dtype"), (dict(tokens=-1), "negative"), (dict(tokens=1 << 41), "many"), (dict(dim=0), "dim"), (dict(dim=16385), "dim"),
+            (dict(sources=0), "sources"), (dict(sources=65), "sources"), (dict(copies=0), "copies"), (dict(copies=65), "copies"),
+            (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(eps=float("inf")), "eps"),
+            (dict(pre_weight=p, pre_dtype=1), "pre_weight"), (dict(post_weight=p, post_dtype=2), "post_weight"), (dict(gate_kind=4), "gate kind"),
+            (dict(gate_kind=1), "gate is null"), (dict(gate_kind=1, gate=p, gate_dtype=1), "gate must"), (dict(residual=None), "residual"),
+            (dict(residual=odd), "aligned"), (dict(post_weight=odd), "aligned")]
+    for k, why in both:
+        refused(sarlib, norm(**k), why)
+        refused(sarlib, norm(backward=True, **k), why)
+    refused(sarlib, norm(pre_weight=p), "go together")
+    refused(sarlib, norm(normed=p), "go together")
+    refused(sarlib, norm(partials=None), "partials")
+    refused(sarlib, norm(sources=1, partials=(ctypes.c_void_p * 1)(None)), "partial")
+    refused(sarlib, norm(total=odd), "aligned")
+    refused(sarlib, L.sar_reduce_norm(0, None, None), "null")
+    assert norm(tokens=0) == 0
+    for g, why in [(dict(grad_normed=p), "without pre_weight"), (dict(grad_pre_weight=p), "without pre_weight"), (dict(grad_post_weight=p), "without post_weight"),
+                   (dict(grad_gate=p), "without a gate"), (dict(total=None), "null"), (dict(total_dtype=2), "total"), (dict(workspace=None), "workspace"),
+                   (dict(workspace_bytes=16), "workspace"), (dict(grad_hidden=odd), "aligned")]:
+        refused(sarlib, norm(backward=True, grads=g), why)
+    refused(sarlib, norm(backward=True, stats=None), "null")
+    assert L.sar_reduce_norm_workspace(4, 8, 0) >= 3 * 8 * 4 and L.sar_reduce_norm_workspace(4, 0, 0) == 0
+
+
+def test_struct_sizes_follow_the_header(tmp_path):
+    """The ctypes structures against what a C compiler makes of the header."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "s.c"
+    src.write_text('#include <stdio.h>\n#include "sar.h"\nint main(void) { printf("%zu %zu %zu %zu\\n", sizeof(sar_reduce_norm_args), '
+                   'offsetof(sar_reduce_norm_args, stats), sizeof(sar_reduce_norm_grads), offsetof(sar_reduce_norm_grads, workspace_bytes)); return 0; }\n')
+    subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(tmp_path / "s")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [ctypes.sizeof(capi.ReduceNormArgs), capi.ReduceNormArgs.stats.offset,
+                   ctypes.sizeof(capi.ReduceNormGrads), capi.ReduceNormGrads.workspace_bytes.offset]
