@@ -12,6 +12,7 @@ them under ``torch.no_grad()`` together with the ``*_backward`` calls, which nee
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple, Optional, Sequence, Union
 
 import torch
@@ -74,7 +75,7 @@ class ReduceNormGrads(NamedTuple):
 
 
 def _tensor(name, t, shape=None, dtypes=None):
-    """Type, shape and layout of an argument; the device comes last so that everything else can be said without one."""
+    """Says what is wrong with an argument; the device comes last so that everything else can be said without one."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a tensor" % name)
     if shape is not None and tuple(t.shape) != tuple(shape):
@@ -87,12 +88,11 @@ def _tensor(name, t, shape=None, dtypes=None):
 
 def _on_device(group, **tensors):
     for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.device.index != group.device):
+        if t is not None and t.get_device() != group.device:
             raise ValueError("%s must be a CUDA tensor on device %d" % (name, group.device))
 
 
-def _stream(group) -> int:
-    return torch.cuda.current_stream(group.device).cuda_stream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _ptr(t):
@@ -101,7 +101,12 @@ def _ptr(t):
 
 def _recording(*tensors) -> bool:
     """Whether autograd has to record the call."""
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            break
+    else:
         return False
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("gradients cannot be recorded while a stream is being captured: call this under torch.no_grad() "
@@ -109,12 +114,29 @@ def _recording(*tensors) -> bool:
     return True
 
 
-def _refuse_captured_backward():
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("the backward pass of a call recorded by autograd cannot be captured: capture the *_backward call")
+class _Node(torch.autograd.Function):
+    """What the recorded calls share: `gradients(ctx, *grads)` is the backward pass.  It is not differentiable itself;
+    the wrapper that says so when somebody tries is only paid for where a graph of the backward pass is asked for."""
+
+    @staticmethod
+    def gradients(ctx, *grads):
+        raise NotImplementedError
+
+    @classmethod
+    def _backward(cls, ctx, *grads):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the backward pass of a call recorded by autograd cannot be captured: capture the *_backward call")
+        if torch.is_grad_enabled():
+            return torch.autograd.function.once_differentiable(cls.gradients)(ctx, *grads)
+        return cls.gradients(ctx, *grads)
 
 
 # ---- route ---------------------------------------------------------------------------------------------------
+
+@functools.lru_cache(maxsize=4096)
+def _route_workspace(tokens, topk, num_experts):
+    return capi.load_library().lib.sar_route_workspace(tokens, topk, num_experts)
+
 
 def route(group, experts, num_experts: int) -> Routing:
     if not isinstance(experts, torch.Tensor) or experts.dim() != 2:
@@ -125,38 +147,40 @@ def route(group, experts, num_experts: int) -> Routing:
         raise ValueError("topk must be 1 to %d, got %d" % (MAX_TOPK, topk))
     if not 1 <= num_experts <= MAX_EXPERTS or num_experts % group.n:
         raise ValueError("num_experts must be a multiple of the %d ranks, at most %d: got %d" % (group.n, MAX_EXPERTS, num_experts))
-    if tokens * topk >= 1 << 31:
+    slots = tokens * topk
+    if slots >= 1 << 31:
         raise ValueError("tokens * topk must stay below 2^31")
     _on_device(group, experts=experts)
-    lib = group._lib
-    slots = tokens * topk
-    # one allocation: row_of_slot, slot_of_row, offsets
-    out = torch.empty(2 * slots + num_experts + 1, dtype=torch.int32, device=experts.device)
-    need = lib.lib.sar_route_workspace(tokens, topk, num_experts)
-    work = torch.empty(need // 4, dtype=torch.int32, device=experts.device) if need else None
-    base = out.data_ptr()
-    lib.check(lib.lib.sar_route(group.device, _stream(group), experts.data_ptr(), experts.element_size(), tokens, topk, num_experts,
-                                base, base + 4 * slots, base + 8 * slots, _ptr(work), need))
-    return Routing(out[:slots].view(tokens, topk), out[slots:2 * slots], out[2 * slots:], num_experts, group.n)
+    lib, device = group._lib, experts.device
+    row_of_slot = torch.empty((tokens, topk), dtype=torch.int32, device=device)
+    slot_of_row = torch.empty(slots, dtype=torch.int32, device=device)
+    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=device)
+    need = _route_workspace(tokens, topk, num_experts)
+    work = torch.empty(need // 4, dtype=torch.int32, device=device) if need else None
+    lib.check(lib.lib.sar_route(group.device, _raw_stream(group.device), experts.data_ptr(), experts.element_size(), tokens, topk, num_experts,
+                                row_of_slot.data_ptr(), slot_of_row.data_ptr(), offsets.data_ptr(), _ptr(work), need))
+    return Routing(row_of_slot, slot_of_row, offsets, num_experts, group.n)
 
 
 # ---- dispatch, combine -----------------------------------------------------------------------------------------
 
 def _dispatch(group, rows, routing, weights=None):
+    tokens, topk = routing.row_of_slot.shape
     dim = rows.shape[1]
-    out = torch.empty(routing.tokens * routing.topk, dim, dtype=rows.dtype, device=rows.device)
+    out = rows.new_empty((tokens * topk, dim))
     lib = group._lib
-    lib.check(lib.lib.sar_dispatch(group.device, _stream(group), DTYPE_CODES[rows.dtype], rows.data_ptr(), routing.tokens, routing.topk, dim,
+    lib.check(lib.lib.sar_dispatch(group.device, _raw_stream(group.device), DTYPE_CODES[rows.dtype], rows.data_ptr(), tokens, topk, dim,
                                    routing.row_of_slot.data_ptr(), routing.offsets.data_ptr(), routing.num_experts,
                                    _ptr(weights), DTYPE_CODES[weights.dtype] if weights is not None else 0, out.data_ptr()))
     return out
 
 
 def _combine(group, rows, routing, weights=None):
+    tokens, topk = routing.row_of_slot.shape
     dim = rows.shape[1]
-    out = torch.empty(routing.tokens, dim, dtype=rows.dtype, device=rows.device)
+    out = rows.new_empty((tokens, dim))
     lib = group._lib
-    lib.check(lib.lib.sar_combine(group.device, _stream(group), DTYPE_CODES[rows.dtype], rows.data_ptr(), routing.tokens, routing.topk, dim,
+    lib.check(lib.lib.sar_combine(group.device, _raw_stream(group.device), DTYPE_CODES[rows.dtype], rows.data_ptr(), tokens, topk, dim,
                                   routing.row_of_slot.data_ptr(), _ptr(weights), DTYPE_CODES[weights.dtype] if weights is not None else 0, out.data_ptr()))
     return out
 
@@ -164,29 +188,32 @@ def _combine(group, rows, routing, weights=None):
 def _combine_backward(group, grad, rows, routing, weights, want_rows, want_weights):
     if not want_weights:
         return (_dispatch(group, grad, routing, weights) if want_rows else None), None
+    tokens, topk = routing.row_of_slot.shape
     grad_rows = torch.empty_like(rows) if want_rows else None
     grad_weights = torch.empty_like(weights)
     lib = group._lib
-    lib.check(lib.lib.sar_combine_backward(group.device, _stream(group), DTYPE_CODES[rows.dtype], grad.data_ptr(), rows.data_ptr(), routing.tokens,
-                                           routing.topk, rows.shape[1], routing.row_of_slot.data_ptr(), routing.offsets.data_ptr(),
+    lib.check(lib.lib.sar_combine_backward(group.device, _raw_stream(group.device), DTYPE_CODES[rows.dtype], grad.data_ptr(), rows.data_ptr(),
+                                           tokens, topk, rows.shape[1], routing.row_of_slot.data_ptr(), routing.offsets.data_ptr(),
                                            routing.num_experts, weights.data_ptr(), DTYPE_CODES[weights.dtype], _ptr(grad_rows), grad_weights.data_ptr()))
     return grad_rows, grad_weights
 
 
-class _Dispatch(torch.autograd.Function):
+class _Dispatch(_Node):
     @staticmethod
     def forward(ctx, rows, group, routing):
         ctx.group, ctx.routing = group, routing
         return _dispatch(group, rows, routing)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        _refuse_captured_backward()
+    def gradients(ctx, grad):
         return _combine(ctx.group, grad.contiguous(), ctx.routing), None, None
 
+    @staticmethod
+    def backward(ctx, grad):
+        return _Dispatch._backward(ctx, grad)
 
-class _Combine(torch.autograd.Function):
+
+class _Combine(_Node):
     @staticmethod
     def forward(ctx, rows, weights, group, routing):
         ctx.group, ctx.routing = group, routing
@@ -194,32 +221,37 @@ class _Combine(torch.autograd.Function):
         return _combine(group, rows, routing, weights)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        _refuse_captured_backward()
+    def gradients(ctx, grad):
         rows, weights = ctx.saved_tensors
-        grads = _combine_backward(ctx.group, grad.contiguous(), rows, ctx.routing, weights, ctx.needs_input_grad[0],
-                                  weights is not None and ctx.needs_input_grad[1])
-        return grads[0], grads[1], None, None
+        need = ctx.needs_input_grad
+        a, b = _combine_backward(ctx.group, grad.contiguous(), rows, ctx.routing, weights, need[0], weights is not None and need[1])
+        return a, b, None, None
+
+    @staticmethod
+    def backward(ctx, grad):
+        return _Combine._backward(ctx, grad)
 
 
-def _check_rows(name, t, rows):
+def _routing_rows(group, name, t, routing, sorted_rows):
+    """The checks of a tensor of rows against a routing."""
+    if not isinstance(routing, Routing):
+        raise TypeError("routing must come from EmulatedGroup.route")
+    tokens, topk = routing.row_of_slot.shape
+    rows = tokens * topk if sorted_rows else tokens
     if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape[0] != rows:
         raise ValueError("%s must be a tensor [%d, dim], got %s" % (name, rows, tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__))
-    _tensor(name, t, dtypes=tuple(DTYPE_CODES))
+    _tensor(name, t, dtypes=DTYPE_CODES)
     if not 1 <= t.shape[1] <= 1 << 24:
         raise ValueError("%s needs 1 to 2^24 columns" % name)
 
 
 def _check_weights(routing, weights, dtype):
     if weights is not None:
-        _tensor("weights", weights, (routing.tokens, routing.topk), (dtype,) if dtype == torch.float32 else (torch.float32, dtype))
+        _tensor("weights", weights, routing.row_of_slot.shape, (torch.float32, dtype))
 
 
 def dispatch(group, tokens, routing):
-    if not isinstance(routing, Routing):
-        raise TypeError("routing must come from EmulatedGroup.route")
-    _check_rows("tokens", tokens, routing.tokens)
+    _routing_rows(group, "tokens", tokens, routing, False)
     _on_device(group, tokens=tokens, routing=routing.offsets)
     if _recording(tokens):
         return _Dispatch.apply(tokens, group, routing)
@@ -227,9 +259,7 @@ def dispatch(group, tokens, routing):
 
 
 def combine(group, rows, routing, weights=None):
-    if not isinstance(routing, Routing):
-        raise TypeError("routing must come from EmulatedGroup.route")
-    _check_rows("rows", rows, routing.tokens * routing.topk)
+    _routing_rows(group, "rows", rows, routing, True)
     _check_weights(routing, weights, rows.dtype)
     _on_device(group, rows=rows, weights=weights, routing=routing.offsets)
     if _recording(rows, weights):
@@ -238,17 +268,13 @@ def combine(group, rows, routing, weights=None):
 
 
 def dispatch_backward(group, grad, routing):
-    if not isinstance(routing, Routing):
-        raise TypeError("routing must come from EmulatedGroup.route")
-    _check_rows("grad", grad, routing.tokens * routing.topk)
+    _routing_rows(group, "grad", grad, routing, True)
     _on_device(group, grad=grad, routing=routing.offsets)
     return _combine(group, grad, routing)
 
 
 def combine_backward(group, grad, rows, routing, weights=None):
-    if not isinstance(routing, Routing):
-        raise TypeError("routing must come from EmulatedGroup.route")
-    _check_rows("rows", rows, routing.tokens * routing.topk)
+    _routing_rows(group, "rows", rows, routing, True)
     _tensor("grad", grad, (routing.tokens, rows.shape[1]), (rows.dtype,))
     _check_weights(routing, weights, rows.dtype)
     _on_device(group, grad=grad, rows=rows, weights=weights, routing=routing.offsets)
@@ -257,113 +283,123 @@ def combine_backward(group, grad, rows, routing, weights=None):
 
 # ---- sum over the ranks, norms, gate, residual -------------------------------------------------------------------
 
-def _reduce_norm(group, partials, residual, pre_weight, post_weight, gate, residual_scale, eps, gather, save):
-    """`partials`: list of tensors [tokens, dim].  Returns hidden, normed (or None), total and stats (or None)."""
+@functools.lru_cache(maxsize=4096)
+def _norm_workspace(tokens, dim, code):
+    return capi.load_library().lib.sar_reduce_norm_workspace(tokens, dim, code)
+
+
+def _norm_args(sources, copies, residual, pre_weight, post_weight, gate, residual_scale, eps, partials=None, hidden=None, normed=None,
+               total=None, stats=None):
+    """sar_reduce_norm_args, by position: dtype, pre_dtype, post_dtype, gate_dtype, gate_kind, sources, copies, reserved, tokens, dim, eps,
+    residual_scale, partials, residual, pre_weight, post_weight, gate, hidden, normed, total, stats."""
     tokens, dim = residual.shape
-    copies = group.n if gather else 1
-    hidden = torch.empty_like(residual)
-    normed = None
+    code = DTYPE_CODES[residual.dtype]
+    pre_code = post_code = gate_code = code
+    kind, pre, post, gate_ptr = _GATE_NONE, None, None, None
     if pre_weight is not None:
-        normed = torch.empty((copies, tokens, dim) if gather else (tokens, dim), dtype=residual.dtype, device=residual.device)
-    total = stats = None
+        pre_code, pre = DTYPE_CODES[pre_weight.dtype], pre_weight.data_ptr()
+    if post_weight is not None:
+        post_code, post = DTYPE_CODES[post_weight.dtype], post_weight.data_ptr()
+    if gate is not None:
+        gate_code, gate_ptr = DTYPE_CODES[gate.dtype], gate.data_ptr()
+        kind = _GATE_CHANNEL if gate.dim() == 1 else _GATE_TOKEN if gate.shape[1] == 1 and dim > 1 else _GATE_FULL
+    return capi.ReduceNormArgs(code, pre_code, post_code, gate_code, kind, sources, copies, 0, tokens, dim, eps, residual_scale, partials,
+                               residual.data_ptr(), pre, post, gate_ptr, hidden, normed, total, stats)
+
+
+def _reduce_norm(group, partials, residual, pre_weight, post_weight, gate, residual_scale, eps, gather, save):
+    """`partials`: sequence of tensors [tokens, dim], or one tensor [n, tokens, dim].  Returns hidden, normed (or None),
+    total and stats (or None)."""
+    tokens, dim = residual.shape
+    if isinstance(partials, torch.Tensor):
+        step, base = tokens * dim * residual.element_size(), partials.data_ptr()
+        addresses = [base + r * step for r in range(partials.shape[0])]
+    else:
+        addresses = [p.data_ptr() for p in partials]
+    sources = len(addresses)
+    hidden = torch.empty_like(residual)
+    normed = total = stats = None
+    if pre_weight is not None:
+        normed = residual.new_empty((group.n, tokens, dim) if gather else (tokens, dim))
     if save:
-        total = partials[0] if len(partials) == 1 else torch.empty(tokens, dim, dtype=torch.float32, device=residual.device)
-        stats = torch.empty(2, tokens, dtype=torch.float32, device=residual.device)
-    args = _norm_args(len(partials), copies, residual, pre_weight, post_weight, gate, residual_scale, eps, stats)
-    args.partials = (ctypes.c_void_p * len(partials))(*[p.data_ptr() for p in partials])
-    args.hidden, args.normed = hidden.data_ptr(), _ptr(normed)
-    args.total = total.data_ptr() if save and len(partials) > 1 else None
+        total = partials[0] if sources == 1 else torch.empty((tokens, dim), dtype=torch.float32, device=residual.device)
+        stats = torch.empty((2, tokens), dtype=torch.float32, device=residual.device)
+    args = _norm_args(sources, group.n if gather else 1, residual, pre_weight, post_weight, gate, residual_scale, eps,
+                      (ctypes.c_void_p * sources)(*addresses), hidden.data_ptr(), _ptr(normed),
+                      total.data_ptr() if save and sources > 1 else None, _ptr(stats))
     lib = group._lib
-    lib.check(lib.lib.sar_reduce_norm(group.device, _stream(group), ctypes.byref(args)))
+    lib.check(lib.lib.sar_reduce_norm(group.device, _raw_stream(group.device), ctypes.byref(args)))
     return hidden, normed, total, stats
 
 
-def _norm_args(sources, copies, residual, pre_weight, post_weight, gate, residual_scale, eps, stats):
-    tokens, dim = residual.shape
-    code = DTYPE_CODES[residual.dtype]
-    args = capi.ReduceNormArgs(dtype=code, pre_dtype=code, post_dtype=code, gate_dtype=code, sources=sources, copies=copies,
-                               tokens=tokens, dim=dim, eps=eps, residual_scale=residual_scale, residual=residual.data_ptr())
-    if pre_weight is not None:
-        args.pre_dtype, args.pre_weight = DTYPE_CODES[pre_weight.dtype], pre_weight.data_ptr()
-    if post_weight is not None:
-        args.post_dtype, args.post_weight = DTYPE_CODES[post_weight.dtype], post_weight.data_ptr()
-    if gate is not None:
-        args.gate_dtype, args.gate = DTYPE_CODES[gate.dtype], gate.data_ptr()
-        args.gate_kind = _GATE_CHANNEL if gate.dim() == 1 else _GATE_TOKEN if gate.shape[1] == 1 and dim > 1 else _GATE_FULL
-    if stats is not None:
-        args.stats = stats.data_ptr()
-    return args
-
-
-def _reduce_norm_backward(group, saved: ReduceNormSaved, grad_hidden, grad_normed, want) -> ReduceNormGrads:
+def _reduce_norm_backward(group, s: ReduceNormSaved, grad_hidden, grad_normed, want) -> ReduceNormGrads:
     """`want`: truth values for partials, residual, pre_weight, post_weight, gate."""
-    s = saved
-    tokens, dim = s.residual.shape
-    dev = s.residual.device
-    args = _norm_args(s.sources, s.copies, s.residual, s.pre_weight, s.post_weight, s.gate, s.residual_scale, s.eps, s.stats)
-    if grad_normed is None or s.pre_weight is None:
-        grad_normed = None
+    residual, pre_weight, post_weight, gate, total = s.residual, s.pre_weight, s.post_weight, s.gate, s.total
+    tokens, dim = residual.shape
+    args = _norm_args(s.sources, s.copies, residual, pre_weight, post_weight, gate, s.residual_scale, s.eps, stats=s.stats.data_ptr())
     out = ReduceNormGrads(
-        torch.empty(s.partial_shape, dtype=s.residual.dtype, device=dev) if want[0] else None,
-        torch.empty_like(s.residual) if want[1] else None,
-        torch.empty_like(s.pre_weight) if want[2] and s.pre_weight is not None else None,
-        torch.empty_like(s.post_weight) if want[3] and s.post_weight is not None else None,
-        torch.empty_like(s.gate) if want[4] and s.gate is not None else None)
+        residual.new_empty(s.partial_shape) if want[0] else None,
+        torch.empty_like(residual) if want[1] else None,
+        torch.empty_like(pre_weight) if want[2] and pre_weight is not None else None,
+        torch.empty_like(post_weight) if want[3] and post_weight is not None else None,
+        torch.empty_like(gate) if want[4] and gate is not None else None)
     lib = group._lib
-    need = lib.lib.sar_reduce_norm_workspace(tokens, dim, args.dtype)
-    work = torch.empty(need // 4, dtype=torch.float32, device=dev)
-    grads = capi.ReduceNormGrads(total=s.total.data_ptr(), total_dtype=DTYPE_CODES[s.total.dtype], grad_hidden=_ptr(grad_hidden),
-                                 grad_normed=_ptr(grad_normed), grad_partials=_ptr(out.partials), grad_residual=_ptr(out.residual),
-                                 grad_pre_weight=_ptr(out.pre_weight), grad_post_weight=_ptr(out.post_weight), grad_gate=_ptr(out.gate),
-                                 workspace=work.data_ptr(), workspace_bytes=need)
-    lib.check(lib.lib.sar_reduce_norm_backward(group.device, _stream(group), ctypes.byref(args), ctypes.byref(grads)))
+    need = _norm_workspace(tokens, dim, args.dtype)
+    work = torch.empty(need // 4, dtype=torch.float32, device=residual.device)
+    # total, total_dtype, reserved, then the gradients that come in, those that go out, and the workspace
+    grads = capi.ReduceNormGrads(total.data_ptr(), DTYPE_CODES[total.dtype], 0, _ptr(grad_hidden), _ptr(grad_normed), _ptr(out[0]), _ptr(out[1]),
+                                 _ptr(out[2]), _ptr(out[3]), _ptr(out[4]), work.data_ptr(), need)
+    lib.check(lib.lib.sar_reduce_norm_backward(group.device, _raw_stream(group.device), ctypes.byref(args), ctypes.byref(grads)))
     return out
 
 
-class _ReduceNorm(torch.autograd.Function):
+class _ReduceNorm(_Node):
     @staticmethod
     def forward(ctx, group, shape, residual_scale, eps, gather, residual, pre_weight, post_weight, gate, *partials):
-        rows = partials if len(shape) == 2 or len(partials) > 1 else partials[0].unbind(0)
+        rows = partials[0] if len(shape) == 3 and len(partials) == 1 else partials
         hidden, normed, total, stats = _reduce_norm(group, rows, residual, pre_weight, post_weight, gate, residual_scale, eps, gather, True)
-        ctx.group, ctx.shape, ctx.sources, ctx.inputs = group, shape, len(rows), len(partials)
-        ctx.options = (residual_scale, eps, gather)
+        ctx.group, ctx.inputs = group, len(partials)
+        ctx.plain = (group.n if len(shape) == 3 else 1, group.n if gather else 1, shape, residual_scale, eps)
         ctx.save_for_backward(total, stats, residual, pre_weight, post_weight, gate)
         ctx.set_materialize_grads(False)
         return hidden, normed
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_hidden, grad_normed):
-        _refuse_captured_backward()
+    def gradients(ctx, grad_hidden, grad_normed):
         total, stats, residual, pre_weight, post_weight, gate = ctx.saved_tensors
-        scale, eps, gather = ctx.options
-        saved = ReduceNormSaved(ctx.sources, ctx.group.n if gather else 1, ctx.shape, total, stats, residual, pre_weight, post_weight, gate, scale, eps)
+        sources, copies, shape, scale, eps = ctx.plain
+        saved = ReduceNormSaved(sources, copies, shape, total, stats, residual, pre_weight, post_weight, gate, scale, eps)
         need = ctx.needs_input_grad
         g = _reduce_norm_backward(ctx.group, saved, grad_hidden.contiguous() if grad_hidden is not None else None,
-                                  grad_normed.contiguous() if grad_normed is not None else None, (any(need[9:]),) + tuple(need[5:9]))
-        if g.partials is None:
+                                  grad_normed.contiguous() if grad_normed is not None else None, (True in need[9:], need[5], need[6], need[7], need[8]))
+        if g[0] is None:
             partials = (None,) * ctx.inputs
         elif ctx.inputs == 1:
-            partials = (g.partials,)
+            partials = (g[0],)
         else:
-            partials = g.partials.unbind(0)
-        return (None,) * 5 + (g.residual, g.pre_weight, g.post_weight, g.gate) + tuple(partials)
+            partials = g[0].unbind(0)
+        return (None, None, None, None, None, g[1], g[2], g[3], g[4], *partials)
+
+    @staticmethod
+    def backward(ctx, grad_hidden, grad_normed):
+        return _ReduceNorm._backward(ctx, grad_hidden, grad_normed)
 
 
 def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], residual, pre_weight=None, post_weight=None, gate=None,
                 residual_scale: float = 1.0, eps: float = 1e-6, gather: bool = True, save: bool = False):
     if not isinstance(residual, torch.Tensor) or residual.dim() != 2:
         raise ValueError("residual must be a tensor [tokens, dim]")
-    _tensor("residual", residual, dtypes=tuple(DTYPE_CODES))
-    tokens, dim = residual.shape
-    dtype = residual.dtype
+    _tensor("residual", residual, dtypes=DTYPE_CODES)
+    size = residual.shape
+    tokens, dim = size
+    dtype, device = residual.dtype, group.device
     if not 1 <= dim <= MAX_NORM_DIM:
         raise ValueError("dim must be 1 to %d, got %d" % (MAX_NORM_DIM, dim))
     if isinstance(partials, torch.Tensor):
         inputs = (partials,)
-        if partials.dim() not in (2, 3) or partials.shape[-2:] != residual.shape or (partials.dim() == 3 and partials.shape[0] != group.n):
+        if partials.dim() not in (2, 3) or partials.shape[-2:] != size or (partials.dim() == 3 and partials.shape[0] != group.n):
             raise ValueError("partials must be [%d ranks, tokens, dim] or, as a finished output, [tokens, dim]: got %s with residual %s"
-                             % (group.n, tuple(partials.shape), tuple(residual.shape)))
+                             % (group.n, tuple(partials.shape), tuple(size)))
         _tensor("partials", partials, dtypes=(dtype,))
         shape = tuple(partials.shape)
     else:
@@ -371,9 +407,10 @@ def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], re
         if len(inputs) != group.n:
             raise ValueError("need one partial output per emulated rank: %d, got %d" % (group.n, len(inputs)))
         for p in inputs:
-            _tensor("a partial output", p, (tokens, dim), (dtype,))
+            if not (isinstance(p, torch.Tensor) and p.dtype is dtype and p.shape == size and p.is_contiguous()):
+                _tensor("a partial output", p, size, (dtype,))
         shape = (group.n, tokens, dim)
-    kinds = (dtype,) if dtype == torch.float32 else (torch.float32, dtype)
+    kinds = (torch.float32, dtype)
     if pre_weight is not None:
         _tensor("pre_weight", pre_weight, (dim,), kinds)
     if post_weight is not None:
@@ -382,21 +419,22 @@ def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], re
         _tensor("gate", gate, dtypes=kinds)
         if tuple(gate.shape) not in ((dim,), (tokens, 1), (tokens, dim)):
             raise ValueError("gate must be [dim], [tokens, 1] or [tokens, dim]: got %s" % (tuple(gate.shape),))
-    if not eps >= 0 or eps == float("inf"):
+    if not 0 <= eps < float("inf"):
         raise ValueError("eps must be a finite number, zero or more")
     _on_device(group, residual=residual, pre_weight=pre_weight, post_weight=post_weight, gate=gate)
     for p in inputs:
-        _on_device(group, partials=p)
+        if p.get_device() != device:
+            _on_device(group, partials=p)
     if _recording(residual, pre_weight, post_weight, gate, *inputs):
         if save:
             raise ValueError("save=True is for calls under torch.no_grad(): autograd keeps what it needs by itself")
-        return _ReduceNorm.apply(group, shape, float(residual_scale), float(eps), bool(gather), residual, pre_weight, post_weight, gate, *inputs)
-    rows = inputs if len(shape) == 2 or len(inputs) > 1 else inputs[0].unbind(0)
+        return _ReduceNorm.apply(group, shape, residual_scale, eps, gather, residual, pre_weight, post_weight, gate, *inputs)
+    rows = partials if len(shape) == 3 and len(inputs) == 1 else inputs
     hidden, normed, total, stats = _reduce_norm(group, rows, residual, pre_weight, post_weight, gate, residual_scale, eps, gather, save)
     if not save:
         return hidden, normed
-    return hidden, normed, ReduceNormSaved(len(rows), group.n if gather else 1, shape, total, stats, residual, pre_weight, post_weight, gate,
-                                           float(residual_scale), float(eps))
+    return hidden, normed, ReduceNormSaved(group.n if len(shape) == 3 else 1, group.n if gather else 1, shape, total, stats, residual,
+                                           pre_weight, post_weight, gate, residual_scale, eps)
 
 
 def reduce_norm_backward(group, saved: ReduceNormSaved, grad_hidden=None, grad_normed=None) -> ReduceNormGrads:

@@ -40,25 +40,61 @@ template <> struct Raw<SAR_F32, 1> { typedef uint32_t T; };
 template <> struct Raw<SAR_F16, 1> { typedef uint16_t T; };
 template <> struct Raw<SAR_BF16, 1> { typedef uint16_t T; };
 
-template <int DT, int VE>
+// NT: streaming, for what nobody reads again soon.
+template <int DT, int VE, bool NT = false>
 __device__ __forceinline__ typename Raw<DT, VE>::T load(const char* base, uint32_t byte) {
     if constexpr (VE == 1) {
         typedef __attribute__((address_space(1))) const typename Raw<DT, VE>::T* P;
         return *(P)(base + byte);
     } else {
         typedef __attribute__((address_space(1))) const u4_any* P;
-        return *(P)(base + byte);
+        return NT ? (u4)__builtin_nontemporal_load((P)(base + byte)) : (u4)*(P)(base + byte);
     }
 }
-template <int DT, int VE>
+template <int DT, int VE, bool NT = false>
 __device__ __forceinline__ void store(char* base, uint32_t byte, typename Raw<DT, VE>::T v) {
     if constexpr (VE == 1) {
         typedef __attribute__((address_space(1))) typename Raw<DT, VE>::T* P;
         *(P)(base + byte) = v;
     } else {
         typedef __attribute__((address_space(1))) u4_any* P;
-        *(P)(base + byte) = v;
+        if (NT) __builtin_nontemporal_store((u4_any)v, (P)(base + byte));
+        else *(P)(base + byte) = v;
     }
+}
+
+// Where a lane's vector `vec` of a row lies.  Behind the row's end it is the last vector again: loads need no branch (a
+// load behind a branch is waited for before the next is issued), sums leave out the first `skip` elements (doubled
+// ones, or all), stores ask `in`.
+template <int DT, int VE>
+struct Place {
+    uint32_t elem, skip;
+    bool in;
+    __device__ __forceinline__ Place(uint32_t vec, uint32_t nvec, uint32_t dim) {
+        elem = min(vec * VE, dim - VE);
+        skip = vec * VE - elem;
+        in = vec < nvec;
+    }
+    __device__ __forceinline__ uint32_t byte() const { return elem * (uint32_t)ElemSize<DT>::value; }
+};
+
+// Loads `count` rows' vectors in batches as large as they come and hands each to `use` in order: all loads of a batch
+// are on their way before the first is waited for.
+template <int N, class Load, class Use>
+__device__ __forceinline__ void batch(uint32_t first, Load&& ld, Use&& use) {
+    decltype(ld(0u)) v[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) v[q] = ld(first + q);
+#pragma unroll
+    for (int q = 0; q < N; ++q) use(v[q]);
+}
+template <int MOST, class Load, class Use>
+__device__ __forceinline__ void in_batches(uint32_t count, Load&& ld, Use&& use) {
+    uint32_t s = 0;
+    for (; s + MOST <= count; s += MOST) batch<MOST>(s, ld, use);
+    if constexpr (MOST > 4) if (s + 4 <= count) { batch<4>(s, ld, use); s += 4; }
+    if constexpr (MOST > 2) if (s + 2 <= count) { batch<2>(s, ld, use); s += 2; }
+    if (s < count) batch<1>(s, ld, use);
 }
 
 __device__ __forceinline__ float widen(uint32_t bits, int dt) {   // one 16-bit element in the low half
@@ -338,7 +374,7 @@ struct MoveArgs {
 };
 
 // Zeros in the rows nobody was sent to: row total + token, and every `tokens`-th behind it.
-template <int DT, int VE, int U>
+template <int DT, int VE, int U, bool NT>
 __device__ __forceinline__ void zero_rows(const MoveArgs& a, uint64_t token, uint32_t v0) {
     uint32_t total = uniform((uint32_t)*a.total);
     if (total > a.nrows) total = a.nrows;
@@ -346,34 +382,36 @@ __device__ __forceinline__ void zero_rows(const MoveArgs& a, uint64_t token, uin
         char* const to = a.out + row * a.row_bytes;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t v = v0 + u * kWave;
-            if (v < a.nvec) store<DT, VE>(to, min(v * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value, typename Raw<DT, VE>::T{});
+            const Place<DT, VE> p(v0 + u * kWave, a.nvec, a.dim);
+            if (p.in) store<DT, VE, NT>(to, p.byte(), typename Raw<DT, VE>::T{});
         }
     }
 }
 
-template <int DT, int VE, int U, bool WEIGHTED>
+__device__ __forceinline__ uint32_t lane_value(uint32_t x, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, lane); }
+__device__ __forceinline__ float lane_value(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
+
+template <int DT, int VE, int U, bool NT, bool WEIGHTED>
 __global__ __launch_bounds__(kMoveThreads) void dispatch_kernel(const MoveArgs a) {
     typedef typename Raw<DT, VE>::T R;
     const uint32_t lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
     const uint32_t v0 = blockIdx.x * (U * kWave) + lane;
     for (uint64_t token = (uint64_t)blockIdx.y * kMoveWaves + wave; token < a.tokens; token += (uint64_t)gridDim.y * kMoveWaves) {
-        const uint64_t slot = token * a.topk + lane;
-        const uint32_t row = lane < a.topk ? (uint32_t)a.row_of_slot[slot] : kDropped;
+        const uint64_t slot = token * a.topk + min(lane, a.topk - 1);
+        const uint32_t listed = (uint32_t)a.row_of_slot[slot];
         float weight = 1.f;
-        if (WEIGHTED && lane < a.topk) weight = load_one<DT>(a.weights, a.weights_f32, slot);
+        if (WEIGHTED) weight = load_one<DT>(a.weights, a.weights_f32, slot);
         const char* const from = a.in + token * a.row_bytes;
         R v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (v0 + u * kWave < a.nvec) v[u] = load<DT, VE>(from, min((v0 + u * kWave) * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value);
-        for (uint64_t left = __ballot(row < a.nrows); left; left &= left - 1) {
+        for (int u = 0; u < U; ++u) v[u] = load<DT, VE, NT>(from, Place<DT, VE>(v0 + u * kWave, a.nvec, a.dim).byte());
+        for (uint64_t left = __ballot(lane < a.topk && listed < a.nrows); left; left &= left - 1) {
             const int k = __builtin_ctzll(left);
-            char* const to = a.out + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)row, k) * a.row_bytes;
-            const float w = WEIGHTED ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), k)) : 1.f;
+            char* const to = a.out + (uint64_t)lane_value(listed, k) * a.row_bytes;
+            const float w = WEIGHTED ? lane_value(weight, k) : 1.f;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (v0 + u * kWave >= a.nvec) continue;
+                const Place<DT, VE> p(v0 + u * kWave, a.nvec, a.dim);
                 R r = v[u];
                 if constexpr (WEIGHTED) {
                     float x[VE];
@@ -382,116 +420,112 @@ __global__ __launch_bounds__(kMoveThreads) void dispatch_kernel(const MoveArgs a
                     for (int i = 0; i < VE; ++i) x[i] *= w;
                     r = pack<DT, VE>(x);
                 }
-                store<DT, VE>(to, min((v0 + u * kWave) * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value, r);
+                if (p.in) store<DT, VE, NT>(to, p.byte(), r);
             }
         }
-        zero_rows<DT, VE, U>(a, token, v0);
+        zero_rows<DT, VE, U, NT>(a, token, v0);
     }
 }
 
-// The sum is kept in 32 bits and taken in the order of the choices; four rows are loaded at a time.
-template <int DT, int VE, int U>
+// The sum is kept in 32 bits and taken in the order of the choices.
+template <int DT, int VE, int U, bool NT>
 __global__ __launch_bounds__(kMoveThreads) void combine_kernel(const MoveArgs a) {
     typedef typename Raw<DT, VE>::T R;
     const uint32_t lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
     const uint32_t v0 = blockIdx.x * (U * kWave) + lane;
+    struct Row { R v[U]; float w; };
     for (uint64_t token = (uint64_t)blockIdx.y * kMoveWaves + wave; token < a.tokens; token += (uint64_t)gridDim.y * kMoveWaves) {
-        const uint64_t slot = token * a.topk + lane;
-        const uint32_t row = lane < a.topk ? (uint32_t)a.row_of_slot[slot] : kDropped;
+        const uint64_t slot = token * a.topk + min(lane, a.topk - 1);
+        const uint32_t listed = (uint32_t)a.row_of_slot[slot];
         float weight = 1.f;
-        if (a.weights && lane < a.topk) weight = load_one<DT>(a.weights, a.weights_f32, slot);
+        if (a.weights) weight = load_one<DT>(a.weights, a.weights_f32, slot);
         float sum[U][VE] = {};
-        uint64_t left = __ballot(row < a.nrows);
-        auto take = [&](auto count) {
-            constexpr int C = decltype(count)::value;
-            R v[C][U];
-            float w[C];
+        uint64_t left = __ballot(lane < a.topk && listed < a.nrows);
+        in_batches<8>((uint32_t)__popcll(left),
+                   [&](uint32_t) {
+                       const int k = __builtin_ctzll(left);
+                       left &= left - 1;
+                       const char* const from = a.in + (uint64_t)lane_value(listed, k) * a.row_bytes;
+                       Row r;
+                       r.w = lane_value(weight, k);
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int k = __builtin_ctzll(left);
-                left &= left - 1;
-                const char* const from = a.in + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)row, k) * a.row_bytes;
-                w[c] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), k));
+                       for (int u = 0; u < U; ++u) r.v[u] = load<DT, VE, NT>(from, Place<DT, VE>(v0 + u * kWave, a.nvec, a.dim).byte());
+                       return r;
+                   },
+                   [&](const Row& r) {
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (v0 + u * kWave < a.nvec) v[c][u] = load<DT, VE>(from, min((v0 + u * kWave) * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value);
-            }
+                       for (int u = 0; u < U; ++u) {
+                           float x[VE];
+                           unpack<DT, VE>(r.v[u], x);
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (v0 + u * kWave >= a.nvec) continue;
-                    float x[VE];
-                    unpack<DT, VE>(v[c][u], x);
-#pragma unroll
-                    for (int i = 0; i < VE; ++i) sum[u][i] = fmaf(w[c], x[i], sum[u][i]);
-                }
-            }
-        };
-        int count = __popcll(left);
-        for (; count >= 4; count -= 4) take(std::integral_constant<int, 4>{});
-        if (count >= 2) { take(std::integral_constant<int, 2>{}); count -= 2; }
-        if (count) take(std::integral_constant<int, 1>{});
+                           for (int i = 0; i < VE; ++i) sum[u][i] = fmaf(r.w, x[i], sum[u][i]);
+                       }
+                   });
         char* const to = a.out + token * a.row_bytes;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (v0 + u * kWave < a.nvec) store<DT, VE>(to, min((v0 + u * kWave) * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value, pack<DT, VE>(sum[u]));
+        for (int u = 0; u < U; ++u) {
+            const Place<DT, VE> p(v0 + u * kWave, a.nvec, a.dim);
+            if (p.in) store<DT, VE, NT>(to, p.byte(), pack<DT, VE>(sum[u]));
+        }
     }
 }
 
 // Both gradients in one pass over the rows: a token's gradient row stays in registers while its rows go by, each read
 // once for its dot product (summed in 32 bits, kept in the lane of its choice) and written once.  SHARE waves take one
 // token's segments in turn where the rows are long; their dot products are added in wave order.
-template <int DT, int VE, int U, int SHARE>
+template <int DT, int VE, int U, int SHARE, bool NT>
 __global__ __launch_bounds__(kMoveThreads) void combine_backward_kernel(const MoveArgs a) {
     typedef typename Raw<DT, VE>::T R;
     __shared__ float dots[kMoveWaves][kWave];
     const uint32_t lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
     const uint32_t part = wave % SHARE;
     constexpr uint32_t kTokens = kMoveWaves / SHARE;            // tokens a workgroup has in hand
+    struct Row { R v[U]; float w; int k; uint64_t at; };
     for (uint64_t base = (uint64_t)blockIdx.x * kTokens; base < a.tokens; base += (uint64_t)gridDim.x * kTokens) {
         const uint64_t token = base + wave / SHARE;
         if (SHARE > 1 || token < a.tokens) {
-            const uint64_t slot = token * a.topk + lane;
-            const uint32_t row = lane < a.topk ? (uint32_t)a.row_of_slot[slot] : kDropped;
-            const float weight = lane < a.topk ? load_one<DT>(a.weights, a.weights_f32, slot) : 0.f;
-            const uint64_t present = __ballot(row < a.nrows);
+            const uint64_t slot = token * a.topk + min(lane, a.topk - 1);
+            const uint32_t listed = (uint32_t)a.row_of_slot[slot];
+            const float weight = load_one<DT>(a.weights, a.weights_f32, slot);
+            const uint64_t present = __ballot(lane < a.topk && listed < a.nrows);
+            const uint32_t count = (uint32_t)__popcll(present);
             const char* const grad = a.in + token * a.row_bytes;
             float dot = 0.f;                                     // of choice `lane`
             for (uint32_t seg = part * (U * kWave); seg < a.nvec; seg += SHARE * U * kWave) {
                 const uint32_t v0 = seg + lane;
-                R g[U];
+                float g[U][VE];
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (v0 + u * kWave < a.nvec) g[u] = load<DT, VE>(grad, min((v0 + u * kWave) * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value);
-                for (uint64_t left = present; left; left &= left - 1) {
-                    const int k = __builtin_ctzll(left);
-                    const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)row, k) * a.row_bytes;
-                    const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), k));
-                    R v[U];
+                for (int u = 0; u < U; ++u) unpack<DT, VE>(load<DT, VE, NT>(grad, Place<DT, VE>(v0 + u * kWave, a.nvec, a.dim).byte()), g[u]);
+                uint64_t left = present;
+                auto ld = [&](uint32_t) {
+                    Row r;
+                    r.k = __builtin_ctzll(left);
+                    left &= left - 1;
+                    r.at = (uint64_t)lane_value(listed, r.k) * a.row_bytes;
+                    r.w = lane_value(weight, r.k);
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (v0 + u * kWave < a.nvec) v[u] = load<DT, VE>(a.rows + at, min((v0 + u * kWave) * VE, a.dim - VE) * (uint32_t)ElemSize<DT>::value);
+                    for (int u = 0; u < U; ++u) r.v[u] = load<DT, VE, NT>(a.rows + r.at, Place<DT, VE>(v0 + u * kWave, a.nvec, a.dim).byte());
+                    return r;
+                };
+                auto use = [&](const Row& r) {
                     float s = 0.f;
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
-                        const uint32_t vec = v0 + u * kWave;
-                        if (vec >= a.nvec) continue;
-                        const uint32_t e0 = min(vec * VE, a.dim - VE), twice = vec * VE - e0;
-                        float x[VE], y[VE];
-                        unpack<DT, VE>(g[u], x);
-                        unpack<DT, VE>(v[u], y);
+                        const Place<DT, VE> p(v0 + u * kWave, a.nvec, a.dim);
+                        float y[VE], x[VE];
+                        unpack<DT, VE>(r.v[u], y);
 #pragma unroll
                         for (int i = 0; i < VE; ++i) {
-                            s = (uint32_t)i >= twice ? fmaf(x[i], y[i], s) : s;
-                            x[i] *= w;
+                            s = (uint32_t)i >= p.skip ? fmaf(g[u][i], y[i], s) : s;
+                            x[i] = g[u][i] * r.w;
                         }
-                        if (a.out) store<DT, VE>(a.out + at, e0 * (uint32_t)ElemSize<DT>::value, pack<DT, VE>(x));
+                        if (a.out && p.in) store<DT, VE, NT>(a.out + r.at, p.byte(), pack<DT, VE>(x));
                     }
                     s = wave_sum(s);
-                    if ((int)lane == k) dot += s;
-                }
-                if (a.out) zero_rows<DT, VE, U>(a, token, v0);
+                    if ((int)lane == r.k) dot += s;
+                };
+                in_batches<4>(count, ld, use);
+                if (a.out) zero_rows<DT, VE, U, NT>(a, token, v0);
             }
             if (SHARE > 1) dots[wave][lane] = dot;
             else if (lane < a.topk) store_one<DT>(a.grad_weights, a.weights_f32, slot, dot);
@@ -527,111 +561,136 @@ struct NormArgs {
 
 constexpr uint32_t kNormThreads = 1024;
 
+// The V vectors of a thread: threadIdx.x, threadIdx.x + blockDim.x, ...
+template <int DT, int VE, int V> struct Vectors { typename Raw<DT, VE>::T v[V]; };
+
+template <int DT, int VE, int V, bool NT = false>
+__device__ __forceinline__ Vectors<DT, VE, V> load_row(const char* row, const NormArgs& a) {
+    Vectors<DT, VE, V> r;
+#pragma unroll
+    for (int v = 0; v < V; ++v) r.v[v] = load<DT, VE, NT>(row, Place<DT, VE>(threadIdx.x + v * blockDim.x, a.nvec, a.dim).byte());
+    return r;
+}
 template <int DT, int VE, int V>
+__device__ __forceinline__ void load_params(const char* p, bool f32, const NormArgs& a, float (&x)[V][VE]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) load_param<DT, VE>(p, f32, Place<DT, VE>(threadIdx.x + v * blockDim.x, a.nvec, a.dim).elem, x[v]);
+}
+template <int V, int VE>
+__device__ __forceinline__ void set(float (&x)[V][VE], float value) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) x[v][i] = value;
+}
+template <int DT, int VE, int V>
+__device__ __forceinline__ void add_row(float (&x)[V][VE], const Vectors<DT, VE, V>& r) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        float y[VE];
+        unpack<DT, VE>(r.v[v], y);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) x[v][i] += y[i];
+    }
+}
+// `count` copies of a row, `step` bytes apart
+template <int DT, int VE, int V, bool NT>
+__device__ __forceinline__ void store_row(char* to, uint64_t step, uint32_t count, const float (&x)[V][VE], const NormArgs& a) {
+    Vectors<DT, VE, V> r;
+#pragma unroll
+    for (int v = 0; v < V; ++v) r.v[v] = pack<DT, VE>(x[v]);
+    for (uint32_t c = 0; c < count; ++c, to += step) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const Place<DT, VE> p(threadIdx.x + v * blockDim.x, a.nvec, a.dim);
+            if (p.in) store<DT, VE, NT>(to, p.byte(), r.v[v]);
+        }
+    }
+}
+// a row in 32 bits, or in DT if f32 is false
+template <int DT, int VE, int V>
+__device__ __forceinline__ void store_params(char* to, bool f32, const float (&x)[V][VE], const NormArgs& a) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const Place<DT, VE> p(threadIdx.x + v * blockDim.x, a.nvec, a.dim);
+        if (!p.in) continue;
+        if (DT == SAR_F32 || f32) {
+            if constexpr (VE == 1) store<SAR_F32, 1>(to, p.elem * 4u, __float_as_uint(x[v][0]));
+            else {
+#pragma unroll
+                for (int q = 0; q < VE / 4; ++q) store<SAR_F32, 4>(to, p.elem * 4u + 16u * q, pack<SAR_F32, 4>(x[v] + 4 * q));
+            }
+        } else {
+            store<DT, VE>(to, p.byte(), pack<DT, VE>(x[v]));
+        }
+    }
+}
+// this thread's part of the sum over a row of x * y, doubled elements once
+template <int DT, int VE, int V>
+__device__ __forceinline__ float dot_row(const float (&x)[V][VE], const float (&y)[V][VE], const NormArgs& a) {
+    float s = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const Place<DT, VE> p(threadIdx.x + v * blockDim.x, a.nvec, a.dim);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) s = (uint32_t)i >= p.skip ? fmaf(x[v][i], y[v][i], s) : s;
+    }
+    return s;
+}
+
+template <int DT, int VE, int V, bool NT>
 __global__ __launch_bounds__(kNormThreads) void reduce_norm_kernel(const NormArgs a) {
-    typedef typename Raw<DT, VE>::T R;
     constexpr uint32_t ES = ElemSize<DT>::value;
+    constexpr bool KEEP = V * VE <= 8;      // weights stay in registers from token to token while that leaves room
     __shared__ float scratch[64];
     BlockSum sum{scratch, 0u, blockDim.x / kWave, uniform(threadIdx.x / kWave), threadIdx.x & (kWave - 1)};
+    float post[V][VE], pre[V][VE], gate[V][VE];
+    if (KEEP) {
+        if (a.post) load_params<DT, VE, V>(a.post, a.post_f32, a, post);
+        if (a.pre) load_params<DT, VE, V>(a.pre, a.pre_f32, a, pre);
+        if (a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, gate);
+    }
     for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
         const uint64_t at = token * a.row_bytes;
+        const auto res = load_row<DT, VE, V, NT>(a.residual + at, a);
+        if (a.gate_kind == SAR_GATE_FULL) load_params<DT, VE, V>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, a, gate);
+        if (a.gate_kind == SAR_GATE_TOKEN) set(gate, load_one<DT>(a.gate, a.gate_f32, token));
         float x[V][VE];
-        R res[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const uint32_t vec = threadIdx.x + v * blockDim.x;
-#pragma unroll
-            for (int i = 0; i < VE; ++i) x[v][i] = 0.f;
-            if (vec >= a.nvec) continue;
-            const uint32_t b = min(vec * VE, a.dim - VE) * ES;
-            res[v] = load<DT, VE>(a.residual + at, b);
-            unpack<DT, VE>(load<DT, VE>(a.partials[0] + at, b), x[v]);
-            uint32_t s = 1;
-            for (; s + 4 <= a.sources; s += 4) {
-                R p[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) p[q] = load<DT, VE>(a.partials[s + q] + at, b);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float y[VE];
-                    unpack<DT, VE>(p[q], y);
-#pragma unroll
-                    for (int i = 0; i < VE; ++i) x[v][i] += y[i];
-                }
-            }
-            for (; s < a.sources; ++s) {
-                float y[VE];
-                unpack<DT, VE>(load<DT, VE>(a.partials[s] + at, b), y);
-#pragma unroll
-                for (int i = 0; i < VE; ++i) x[v][i] += y[i];
-            }
-            if (a.total) {
-                char* const t = (char*)a.total + token * a.dim * 4u;
-                if constexpr (VE == 1) store<SAR_F32, 1>(t, b / ES * 4u, __float_as_uint(x[v][0]));
-                else {
-#pragma unroll
-                    for (int q = 0; q < VE / 4; ++q) store<SAR_F32, 4>(t, b / ES * 4u + 16u * q, pack<SAR_F32, 4>(x[v] + 4 * q));
-                }
-            }
-        }
+        set(x, 0.f);
+        in_batches<8 / V>(a.sources, [&](uint32_t s) { return load_row<DT, VE, V, NT>(a.partials[s] + at, a); },
+                   [&](const Vectors<DT, VE, V>& r) { add_row<DT, VE, V>(x, r); });
+        if (a.total) store_params<DT, VE, V>((char*)(a.total + token * a.dim), true, x, a);
         float r1 = 1.f;
         if (a.post) {
-            float ss = 0.f;
+            r1 = dot_row<DT, VE, V>(x, x, a);
+            sum(r1);
+            r1 = rsqrtf(fmaf(r1, a.inv_dim, a.eps));
+            if (!KEEP) load_params<DT, VE, V>(a.post, a.post_f32, a, post);
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const uint32_t vec = threadIdx.x + v * blockDim.x;
-                const uint32_t twice = vec < a.nvec ? vec * VE - min(vec * VE, a.dim - VE) : 0u;
+            for (int v = 0; v < V; ++v)
 #pragma unroll
-                for (int i = 0; i < VE; ++i) ss = (uint32_t)i >= twice ? fmaf(x[v][i], x[v][i], ss) : ss;
-            }
-            sum(ss);
-            r1 = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
+                for (int i = 0; i < VE; ++i) x[v][i] = x[v][i] * r1 * post[v][i];
         }
-        const float token_gate = a.gate_kind == SAR_GATE_TOKEN ? load_one<DT>(a.gate, a.gate_f32, token) : 1.f;
-        float ss = 0.f;
+        if (!KEEP && a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, gate);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const uint32_t vec = threadIdx.x + v * blockDim.x;
-            if (vec >= a.nvec) continue;
-            const uint32_t e0 = min(vec * VE, a.dim - VE), twice = vec * VE - e0;
-            float h[VE], w[VE];
-            unpack<DT, VE>(res[v], h);
-            if (a.post) {
-                load_param<DT, VE>(a.post, a.post_f32, e0, w);
+            float h[VE];
+            unpack<DT, VE>(res.v[v], h);
 #pragma unroll
-                for (int i = 0; i < VE; ++i) x[v][i] = x[v][i] * r1 * w[i];
-            }
-            if (a.gate_kind == SAR_GATE_CHANNEL || a.gate_kind == SAR_GATE_FULL) {
-                const uint64_t skip = a.gate_kind == SAR_GATE_FULL ? token * a.dim * (a.gate_f32 ? 4u : ES) : 0u;
-                load_param<DT, VE>(a.gate + skip, a.gate_f32, e0, w);
-            } else {
-#pragma unroll
-                for (int i = 0; i < VE; ++i) w[i] = token_gate;
-            }
-#pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                x[v][i] = fmaf(a.residual_scale, h[i], w[i] * x[v][i]);
-                ss = (uint32_t)i >= twice ? fmaf(x[v][i], x[v][i], ss) : ss;
-            }
-            if (a.hidden) store<DT, VE>(a.hidden + at, e0 * ES, pack<DT, VE>(x[v]));
+            for (int i = 0; i < VE; ++i) x[v][i] = fmaf(a.residual_scale, h[i], a.gate_kind == SAR_GATE_NONE ? x[v][i] : gate[v][i] * x[v][i]);
         }
+        if (a.hidden) store_row<DT, VE, V, NT>(a.hidden + at, 0, 1, x, a);
         float r2 = 1.f;
         if (a.pre) {
-            sum(ss);
-            r2 = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
+            r2 = dot_row<DT, VE, V>(x, x, a);
+            sum(r2);
+            r2 = rsqrtf(fmaf(r2, a.inv_dim, a.eps));
+            if (!KEEP) load_params<DT, VE, V>(a.pre, a.pre_f32, a, pre);
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const uint32_t vec = threadIdx.x + v * blockDim.x;
-                if (vec >= a.nvec) continue;
-                const uint32_t e0 = min(vec * VE, a.dim - VE);
-                float w[VE];
-                load_param<DT, VE>(a.pre, a.pre_f32, e0, w);
+            for (int v = 0; v < V; ++v)
 #pragma unroll
-                for (int i = 0; i < VE; ++i) x[v][i] = x[v][i] * r2 * w[i];
-                const R r = pack<DT, VE>(x[v]);
-                char* to = a.normed + at;
-                for (uint32_t c = 0; c < a.copies; ++c, to += a.copy_bytes) store<DT, VE>(to, e0 * ES, r);
-            }
+                for (int i = 0; i < VE; ++i) x[v][i] = x[v][i] * r2 * pre[v][i];
+            store_row<DT, VE, V, NT>(a.normed + at, a.copy_bytes, a.copies, x, a);
         }
         if (a.stats && threadIdx.x == 0) { a.stats[token] = r1; a.stats[a.tokens + token] = r2; }
     }
@@ -656,157 +715,102 @@ struct NormBackwardArgs {
     uint32_t total_f32, want_pre, want_post, want_gate;   // want_gate: a channel gate's
 };
 
-template <int DT, int VE, int V>
+template <int DT, int VE, int V, bool NT>
 __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(const NormBackwardArgs b) {
-    typedef typename Raw<DT, VE>::T R;
     constexpr uint32_t ES = ElemSize<DT>::value;
     __shared__ float scratch[64];
     const NormArgs& a = b.f;
     BlockSum sum{scratch, 0u, blockDim.x / kWave, uniform(threadIdx.x / kWave), threadIdx.x & (kWave - 1)};
-    float col_pre[V][VE] = {}, col_post[V][VE] = {}, col_gate[V][VE] = {};
+    float col_pre[V][VE], col_post[V][VE], col_gate[V][VE];
+    set(col_pre, 0.f), set(col_post, 0.f), set(col_gate, 0.f);
     for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
         const uint64_t at = token * a.row_bytes;
         const float r1 = a.stats[token], r2 = a.stats[a.tokens + token];
         const float token_gate = a.gate_kind == SAR_GATE_TOKEN ? load_one<DT>(a.gate, a.gate_f32, token) : 1.f;
+        const auto res = load_row<DT, VE, V, NT>(a.residual + at, a);
+        Vectors<DT, VE, V> gh{};
+        if (b.grad_hidden) gh = load_row<DT, VE, V, NT>(b.grad_hidden + at, a);
         float y[V][VE];      // yhat (y without a norm there)
-        float h[V][VE];      // hhat
-        float d[V][VE];      // G pre, then d hidden
-        float mean = 0.f;
+        load_params<DT, VE, V>(b.total + token * a.dim * (b.total_f32 ? 4u : ES), b.total_f32, a, y);
+        float d[V][VE];      // G, then G pre, then d hidden
+        set(d, 0.f);
+        if (b.grad_normed)
+            in_batches<V == 1 ? 4 : 8 / V>(a.copies, [&](uint32_t c) { return load_row<DT, VE, V, NT>(b.grad_normed + at + c * a.copy_bytes, a); },
+                       [&](const Vectors<DT, VE, V>& r) { add_row<DT, VE, V>(d, r); });
+        float post[V][VE], gate[V][VE], h[V][VE];      // h: hhat
+        if (a.post) load_params<DT, VE, V>(a.post, a.post_f32, a, post);
+        else set(post, 1.f);
+        if (a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, gate);
+        else if (a.gate_kind == SAR_GATE_FULL) load_params<DT, VE, V>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, a, gate);
+        else set(gate, token_gate);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const uint32_t vec = threadIdx.x + v * blockDim.x;
+            unpack<DT, VE>(res.v[v], h[v]);
 #pragma unroll
-            for (int i = 0; i < VE; ++i) y[v][i] = h[v][i] = d[v][i] = 0.f;
-            if (vec >= a.nvec) continue;
-            const uint32_t e0 = min(vec * VE, a.dim - VE), twice = vec * VE - e0;
-            load_param<DT, VE>(b.total + token * a.dim * (b.total_f32 ? 4u : ES), b.total_f32, e0, y[v]);
-            unpack<DT, VE>(load<DT, VE>(a.residual + at, e0 * ES), h[v]);
-            if (b.grad_normed) {
-                const char* from = b.grad_normed + at;
-                uint32_t c = 0;
-                for (; c + 4 <= a.copies; c += 4, from += 4 * a.copy_bytes) {
-                    R p[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) p[q] = load<DT, VE>(from + q * a.copy_bytes, e0 * ES);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        float x[VE];
-                        unpack<DT, VE>(p[q], x);
-#pragma unroll
-                        for (int i = 0; i < VE; ++i) d[v][i] += x[i];
-                    }
-                }
-                for (; c < a.copies; ++c, from += a.copy_bytes) {
-                    float x[VE];
-                    unpack<DT, VE>(load<DT, VE>(from, e0 * ES), x);
-#pragma unroll
-                    for (int i = 0; i < VE; ++i) d[v][i] += x[i];
-                }
-            }
-            float w[VE], g[VE];
-#pragma unroll
-            for (int i = 0; i < VE; ++i) { w[i] = 1.f; g[i] = token_gate; y[v][i] *= r1; }
-            if (a.post) load_param<DT, VE>(a.post, a.post_f32, e0, w);
-            if (a.gate_kind == SAR_GATE_CHANNEL) load_param<DT, VE>(a.gate, a.gate_f32, e0, g);
-            if (a.gate_kind == SAR_GATE_FULL) load_param<DT, VE>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, e0, g);
-#pragma unroll
-            for (int i = 0; i < VE; ++i) h[v][i] = fmaf(a.residual_scale, h[v][i], g[i] * (y[v][i] * w[i])) * r2;
-            if (b.grad_normed) {
-                load_param<DT, VE>(a.pre, a.pre_f32, e0, w);
-#pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    col_pre[v][i] = fmaf(d[v][i], h[v][i], col_pre[v][i]);
-                    d[v][i] *= w[i];
-                    mean = (uint32_t)i >= twice ? fmaf(d[v][i], h[v][i], mean) : mean;
-                }
+            for (int i = 0; i < VE; ++i) {
+                y[v][i] *= r1;
+                h[v][i] = fmaf(a.residual_scale, h[v][i], gate[v][i] * (y[v][i] * post[v][i])) * r2;
             }
         }
         if (b.grad_normed) {
+            float pre[V][VE];
+            load_params<DT, VE, V>(a.pre, a.pre_f32, a, pre);
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    col_pre[v][i] = fmaf(d[v][i], h[v][i], col_pre[v][i]);
+                    d[v][i] *= pre[v][i];
+                }
+            float mean = dot_row<DT, VE, V>(d, h, a);
             sum(mean);
             mean *= a.inv_dim;
-        }
-        float dot = 0.f, gate_dot = 0.f;
-        float t[V][VE];      // du post
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const uint32_t vec = threadIdx.x + v * blockDim.x;
-            if (vec >= a.nvec) continue;
-            const uint32_t e0 = min(vec * VE, a.dim - VE), twice = vec * VE - e0;
-            if (b.grad_normed) {
+            for (int v = 0; v < V; ++v)
 #pragma unroll
                 for (int i = 0; i < VE; ++i) d[v][i] = r2 * fmaf(-h[v][i], mean, d[v][i]);
-            }
-            float w[VE], g[VE], x[VE];
-            if (b.grad_hidden) {
-                unpack<DT, VE>(load<DT, VE>(b.grad_hidden + at, e0 * ES), x);
+        }
+        if (b.grad_hidden) add_row<DT, VE, V>(d, gh);
+        if (b.grad_residual) {
 #pragma unroll
-                for (int i = 0; i < VE; ++i) d[v][i] += x[i];
-            }
-            if (b.grad_residual) {
+            for (int v = 0; v < V; ++v)
 #pragma unroll
-                for (int i = 0; i < VE; ++i) x[i] = a.residual_scale * d[v][i];
-                store<DT, VE>(b.grad_residual + at, e0 * ES, pack<DT, VE>(x));
-            }
+                for (int i = 0; i < VE; ++i) h[v][i] = a.residual_scale * d[v][i];
+            store_row<DT, VE, V, NT>(b.grad_residual + at, 0, 1, h, a);
+        }
+        float gate_dot = 0.f;
 #pragma unroll
-            for (int i = 0; i < VE; ++i) { w[i] = 1.f; g[i] = token_gate; }
-            if (a.post) load_param<DT, VE>(a.post, a.post_f32, e0, w);
-            if (a.gate_kind == SAR_GATE_CHANNEL) load_param<DT, VE>(a.gate, a.gate_f32, e0, g);
-            if (a.gate_kind == SAR_GATE_FULL) load_param<DT, VE>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, e0, g);
+        for (int v = 0; v < V; ++v) {
+            const Place<DT, VE> p(threadIdx.x + v * blockDim.x, a.nvec, a.dim);
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
-                const float du = d[v][i] * g[i];
-                x[i] = d[v][i] * (y[v][i] * w[i]);
-                col_gate[v][i] += x[i];
+                const float du = d[v][i] * gate[v][i];
+                h[v][i] = d[v][i] * (y[v][i] * post[v][i]);                  // gradient of the gate
+                col_gate[v][i] += h[v][i];
                 col_post[v][i] = fmaf(du, y[v][i], col_post[v][i]);
-                t[v][i] = du * w[i];
-                dot = (uint32_t)i >= twice ? fmaf(t[v][i], y[v][i], dot) : dot;
-                gate_dot += (uint32_t)i >= twice ? x[i] : 0.f;
-            }
-            if (a.gate_kind == SAR_GATE_FULL && b.grad_gate) {
-                char* const to = b.grad_gate + token * a.dim * (a.gate_f32 ? 4u : ES);
-                if (DT == SAR_F32 || a.gate_f32) {
-                    if constexpr (VE == 1) store<SAR_F32, 1>(to, e0 * 4u, __float_as_uint(x[0]));
-                    else {
-#pragma unroll
-                        for (int q = 0; q < VE / 4; ++q) store<SAR_F32, 4>(to, e0 * 4u + 16u * q, pack<SAR_F32, 4>(x + 4 * q));
-                    }
-                } else {
-                    store<DT, VE>(to, e0 * ES, pack<DT, VE>(x));
-                }
+                d[v][i] = du * post[v][i];
+                gate_dot += (uint32_t)i >= p.skip ? h[v][i] : 0.f;
             }
         }
-        sum(dot, gate_dot);
+        if (a.gate_kind == SAR_GATE_FULL && b.grad_gate) store_params<DT, VE, V>(b.grad_gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, h, a);
+        if (a.post) {
+            float mean = dot_row<DT, VE, V>(d, y, a);
+            sum(mean, gate_dot);
+            mean *= a.inv_dim;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+#pragma unroll
+                for (int i = 0; i < VE; ++i) d[v][i] = r1 * fmaf(-y[v][i], mean, d[v][i]);
+        } else if (a.gate_kind == SAR_GATE_TOKEN) {
+            sum(gate_dot);
+        }
         if (a.gate_kind == SAR_GATE_TOKEN && b.grad_gate && threadIdx.x == 0) store_one<DT>(b.grad_gate, a.gate_f32, token, gate_dot);
-        if (b.grad_partials) {
-            dot *= a.inv_dim;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const uint32_t vec = threadIdx.x + v * blockDim.x;
-                if (vec >= a.nvec) continue;
-                const uint32_t e0 = min(vec * VE, a.dim - VE);
-                if (a.post) {
-#pragma unroll
-                    for (int i = 0; i < VE; ++i) t[v][i] = r1 * fmaf(-y[v][i], dot, t[v][i]);
-                }
-                const R r = pack<DT, VE>(t[v]);
-                char* to = b.grad_partials + at;
-                for (uint32_t s = 0; s < a.sources; ++s, to += a.copy_bytes) store<DT, VE>(to, e0 * ES, r);
-            }
-        }
+        if (b.grad_partials) store_row<DT, VE, V, NT>(b.grad_partials + at, a.copy_bytes, a.sources, d, a);
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const uint32_t vec = threadIdx.x + v * blockDim.x;
-        if (vec >= a.nvec) continue;
-        const uint32_t e0 = min(vec * VE, a.dim - VE);
-        float* const to = b.columns + (uint64_t)blockIdx.x * 3u * a.dim + e0;
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            if (b.want_pre) to[i] = col_pre[v][i];
-            if (b.want_post) to[a.dim + i] = col_post[v][i];
-            if (b.want_gate) to[2 * a.dim + i] = col_gate[v][i];
-        }
-    }
+    char* const columns = (char*)(b.columns + (uint64_t)blockIdx.x * 3u * a.dim);
+    if (b.want_pre) store_params<DT, VE, V>(columns, true, col_pre, a);
+    if (b.want_post) store_params<DT, VE, V>(columns + (uint64_t)a.dim * 4u, true, col_post, a);
+    if (b.want_gate) store_params<DT, VE, V>(columns + (uint64_t)a.dim * 8u, true, col_gate, a);
 }
 
 // Adds the workgroups' rows of column sums: 64 columns a workgroup, 16 waves taking every 16th row, then in wave order.
@@ -923,11 +927,24 @@ MoveArgs move_args(int dtype, int64_t tokens, int topk, int64_t dim, const int32
     return a;
 }
 
-// Vectors per lane: four where that still leaves every CU its waves, one where there are few tokens (the smallest
+// Calls that move this much and more stream their rows past the caches: what does not fit into the 256 MB Infinity
+// Cache only pushes out what does, and a cached store's way to memory is paid for by the next call.  Measured, cached
+// against streaming, as a chain with a pass over the result behind it: dispatch of 537 MB 407 against 381 us (chain
+// with its combine), of 268 MB 173 against 184; eight partials of 8192 x 4096 (1.2 GB) 432 against 397, of 4096 222
+// against 213, of 2048 (302 MB) 107 against 118.
+constexpr uint64_t kStreamBytes = 512ull << 20;
+
+// calls f(integral_constant<bool, B>)
+template <class F> void with_bool(bool b, F&& f) {
+    if (b) f(std::true_type{});
+    else f(std::false_type{});
+}
+
+// Vectors per lane: several where that still leaves every CU its waves, one where there are few tokens (the smallest
 // calls are bound by the time of one trip to memory, and more waves make it one trip instead of four).
-int move_vectors(const MoveArgs& a) {
-    const uint64_t segments = (a.nvec + 4 * kWave - 1) / (4 * kWave);
-    return a.tokens * segments >= 4096 && a.nvec > kWave ? 4 : 1;
+bool many_vectors(const MoveArgs& a, uint32_t u) {
+    const uint64_t segments = (a.nvec + u * kWave - 1) / (u * kWave);
+    return a.tokens * segments >= 4096 && a.nvec > kWave;
 }
 
 dim3 move_grid(const MoveArgs& a, int u) {
@@ -935,36 +952,43 @@ dim3 move_grid(const MoveArgs& a, int u) {
     return dim3((a.nvec + u * kWave - 1) / (u * kWave), (uint32_t)std::min<uint64_t>(groups, 65535u));
 }
 
+constexpr int kDispatchVectors = 4, kCombineVectors = 2;
+
 template <int DT> void launch_dispatch(hipStream_t st, const MoveArgs& a) {
-    const int u = move_vectors(a);
-    const dim3 grid = move_grid(a, u);
-    if (a.dim < kVec<DT>) {
-        if (a.weights) dispatch_kernel<DT, 1, 1, true><<<grid, kMoveThreads, 0, st>>>(a);
-        else dispatch_kernel<DT, 1, 1, false><<<grid, kMoveThreads, 0, st>>>(a);
-    } else if (u == 4) {
-        if (a.weights) dispatch_kernel<DT, kVec<DT>, 4, true><<<grid, kMoveThreads, 0, st>>>(a);
-        else dispatch_kernel<DT, kVec<DT>, 4, false><<<grid, kMoveThreads, 0, st>>>(a);
-    } else {
-        if (a.weights) dispatch_kernel<DT, kVec<DT>, 1, true><<<grid, kMoveThreads, 0, st>>>(a);
-        else dispatch_kernel<DT, kVec<DT>, 1, false><<<grid, kMoveThreads, 0, st>>>(a);
-    }
+    const bool nt = ((uint64_t)a.nrows + a.tokens) * a.row_bytes >= kStreamBytes;
+    with_bool(a.weights != nullptr, [&](auto weighted) {
+        constexpr bool W = decltype(weighted)::value;
+        constexpr int U = kDispatchVectors;
+        if (a.dim < kVec<DT>) dispatch_kernel<DT, 1, 1, false, W><<<move_grid(a, 1), kMoveThreads, 0, st>>>(a);
+        else if (!many_vectors(a, U)) dispatch_kernel<DT, kVec<DT>, 1, false, W><<<move_grid(a, 1), kMoveThreads, 0, st>>>(a);
+        else if (nt) dispatch_kernel<DT, kVec<DT>, U, true, W><<<move_grid(a, U), kMoveThreads, 0, st>>>(a);
+        else dispatch_kernel<DT, kVec<DT>, U, false, W><<<move_grid(a, U), kMoveThreads, 0, st>>>(a);
+    });
 }
 
 template <int DT> void launch_combine(hipStream_t st, const MoveArgs& a) {
-    const int u = move_vectors(a);
-    const dim3 grid = move_grid(a, u);
-    if (a.dim < kVec<DT>) combine_kernel<DT, 1, 1><<<grid, kMoveThreads, 0, st>>>(a);
-    else if (u == 4) combine_kernel<DT, kVec<DT>, 4><<<grid, kMoveThreads, 0, st>>>(a);
-    else combine_kernel<DT, kVec<DT>, 1><<<grid, kMoveThreads, 0, st>>>(a);
+    const bool nt = ((uint64_t)a.nrows + a.tokens) * a.row_bytes >= kStreamBytes;
+    constexpr int U = kCombineVectors;
+    if (a.dim < kVec<DT>) combine_kernel<DT, 1, 1, false><<<move_grid(a, 1), kMoveThreads, 0, st>>>(a);
+    else if (!many_vectors(a, U)) combine_kernel<DT, kVec<DT>, 1, false><<<move_grid(a, 1), kMoveThreads, 0, st>>>(a);
+    else if (nt) combine_kernel<DT, kVec<DT>, U, true><<<move_grid(a, U), kMoveThreads, 0, st>>>(a);
+    else combine_kernel<DT, kVec<DT>, U, false><<<move_grid(a, U), kMoveThreads, 0, st>>>(a);
 }
 
 template <int DT> void launch_combine_backward(hipStream_t st, const MoveArgs& a) {
     const bool shared = a.nvec > 4 * kWave;
     const uint64_t groups = shared ? a.tokens : (a.tokens + kMoveWaves - 1) / kMoveWaves;
     const uint32_t grid = (uint32_t)std::min<uint64_t>(groups, 1u << 20);
-    if (a.dim < kVec<DT>) combine_backward_kernel<DT, 1, 1, 1><<<grid, kMoveThreads, 0, st>>>(a);
-    else if (shared) combine_backward_kernel<DT, kVec<DT>, 2, 4><<<grid, kMoveThreads, 0, st>>>(a);
-    else combine_backward_kernel<DT, kVec<DT>, 4, 1><<<grid, kMoveThreads, 0, st>>>(a);
+    const bool nt = ((uint64_t)a.nrows * (a.out ? 2 : 1) + a.tokens) * a.row_bytes >= kStreamBytes;
+    if (a.dim < kVec<DT>) {
+        combine_backward_kernel<DT, 1, 1, 1, false><<<grid, kMoveThreads, 0, st>>>(a);
+        return;
+    }
+    with_bool(nt, [&](auto stream) {
+        constexpr bool NT = decltype(stream)::value;
+        if (shared) combine_backward_kernel<DT, kVec<DT>, 2, 4, NT><<<grid, kMoveThreads, 0, st>>>(a);
+        else combine_backward_kernel<DT, kVec<DT>, 4, 1, NT><<<grid, kMoveThreads, 0, st>>>(a);
+    });
 }
 
 // Threads and vectors per thread for a row: one vector a thread as far as 1024 threads reach.
@@ -1036,19 +1060,29 @@ NormArgs norm_args(const sar_reduce_norm_args* a) {
     return k;
 }
 
-template <int DT> void launch_norm(hipStream_t st, const NormArgs& a, const NormShape& s) {
-    const uint32_t grid = (uint32_t)std::min<uint64_t>(a.tokens, 1u << 20);
-    if (s.single) reduce_norm_kernel<DT, 1, 1><<<grid, s.threads, 0, st>>>(a);
-    else if (s.vectors == 1) reduce_norm_kernel<DT, kVec<DT>, 1><<<grid, s.threads, 0, st>>>(a);
-    else if (s.vectors == 2) reduce_norm_kernel<DT, kVec<DT>, 2><<<grid, s.threads, 0, st>>>(a);
-    else if constexpr (DT == SAR_F32) reduce_norm_kernel<DT, kVec<DT>, 4><<<grid, s.threads, 0, st>>>(a);
+// calls f(integral_constant<int, VE>, integral_constant<int, V>) for a shape
+template <int DT, class F> void with_norm_shape(const NormShape& s, F&& f) {
+    using std::integral_constant;
+    if (s.single) f(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    else if (s.vectors == 1) f(integral_constant<int, kVec<DT>>{}, integral_constant<int, 1>{});
+    else if (s.vectors == 2) f(integral_constant<int, kVec<DT>>{}, integral_constant<int, 2>{});
+    else if constexpr (DT == SAR_F32) f(integral_constant<int, kVec<DT>>{}, integral_constant<int, 4>{});
 }
 
-template <int DT> void launch_norm_backward(hipStream_t st, const NormBackwardArgs& a, const NormShape& s, uint32_t grid) {
-    if (s.single) reduce_norm_backward_kernel<DT, 1, 1><<<grid, s.threads, 0, st>>>(a);
-    else if (s.vectors == 1) reduce_norm_backward_kernel<DT, kVec<DT>, 1><<<grid, s.threads, 0, st>>>(a);
-    else if (s.vectors == 2) reduce_norm_backward_kernel<DT, kVec<DT>, 2><<<grid, s.threads, 0, st>>>(a);
-    else if constexpr (DT == SAR_F32) reduce_norm_backward_kernel<DT, kVec<DT>, 4><<<grid, s.threads, 0, st>>>(a);
+template <int DT> void launch_norm(hipStream_t st, const NormArgs& a, const NormShape& s) {
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(a.tokens, 1u << 20);
+    const uint64_t rows = a.sources + 2 + (a.normed ? a.copies : 0) + (a.total ? 4 / ElemSize<DT>::value : 0);
+    with_bool(rows * a.copy_bytes >= kStreamBytes, [&](auto nt) {
+        with_norm_shape<DT>(s, [&](auto ve, auto v) { reduce_norm_kernel<DT, decltype(ve)::value, decltype(v)::value, decltype(nt)::value><<<grid, s.threads, 0, st>>>(a); });
+    });
+}
+
+template <int DT> void launch_norm_backward(hipStream_t st, const NormBackwardArgs& b, const NormShape& s, uint32_t grid) {
+    const NormArgs& a = b.f;
+    const uint64_t rows = (b.grad_partials ? a.sources : 0) + 3 + (b.grad_normed ? a.copies : 0) + (b.total_f32 ? 4 / ElemSize<DT>::value : 1);
+    with_bool(rows * a.copy_bytes >= kStreamBytes, [&](auto nt) {
+        with_norm_shape<DT>(s, [&](auto ve, auto v) { reduce_norm_backward_kernel<DT, decltype(ve)::value, decltype(v)::value, decltype(nt)::value><<<grid, s.threads, 0, st>>>(b); });
+    });
 }
 
 }  // namespace
