@@ -407,7 +407,7 @@ def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], re
         if len(inputs) != group.n:
             raise ValueError("need one partial output per emulated rank: %d, got %d" % (group.n, len(inputs)))
         for p in inputs:
-            if not (isinstance(p, torch.Tensor) and p.dtype is dtype and p.shape == size and p.is_contiguous()):
+            if not isinstance(p, torch.Tensor) or p.dtype is not dtype or p.shape != size or not p.is_contiguous():
                 _tensor("a partial output", p, size, (dtype,))
         shape = (group.n, tokens, dim)
     kinds = (torch.float32, dtype)
@@ -421,10 +421,9 @@ def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], re
             raise ValueError("gate must be [dim], [tokens, 1] or [tokens, dim]: got %s" % (tuple(gate.shape),))
     if not 0 <= eps < float("inf"):
         raise ValueError("eps must be a finite number, zero or more")
-    _on_device(group, residual=residual, pre_weight=pre_weight, post_weight=post_weight, gate=gate)
-    for p in inputs:
-        if p.get_device() != device:
-            _on_device(group, partials=p)
+    for t in (residual, pre_weight, post_weight, gate) + inputs:
+        if t is not None and t.get_device() != device:
+            raise ValueError("every tensor must be a CUDA tensor on device %d" % device)
     if _recording(residual, pre_weight, post_weight, gate, *inputs):
         if save:
             raise ValueError("save=True is for calls under torch.no_grad(): autograd keeps what it needs by itself")

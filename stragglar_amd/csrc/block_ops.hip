@@ -229,12 +229,15 @@ __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__bui
 // A stable counting sort.  A wave takes strips of 64 consecutive slots; lanes with the same expert find each other by
 // one ballot per bit of the expert number, so a slot's place among its equals in the strip is a population count, and
 // the wave's running count of each expert sits in LDS.  Nothing depends on the order in which waves arrive.
-// Up to kRouteOne slots one workgroup does it all in one launch; above, one launch counts the slots of each expert in
-// every block of kRouteBlock slots, one turns the counts into first rows, and one places the slots.
+// Few slots: one workgroup does it all in one launch.  More: one launch counts the slots of each expert in every block
+// of kRouteBlock slots and one places them, every block adding up the counts of the blocks before it.  Many blocks:
+// that sum, which grows with the square of the blocks, becomes a launch of its own.
 constexpr uint32_t kRouteThreads = 1024, kRouteWaves = kRouteThreads / kWave;
 constexpr uint32_t kRouteOneStrips = 8, kRouteStrips = 4;
 constexpr uint32_t kRouteOne = kRouteThreads * kRouteOneStrips, kRouteBlock = kRouteThreads * kRouteStrips;
+constexpr uint64_t kRouteSumMost = 16384;   // counts that a block adds up itself, at most
 constexpr uint32_t kDropped = 0xffffffffu;
+enum { kRouteAlone, kRouteSum, kRouteScanned };   // where a block's first rows come from
 
 template <typename I>
 __device__ __forceinline__ uint32_t slot_expert(const I* experts, uint32_t n, uint32_t slot, uint32_t num_experts) {
@@ -243,21 +246,22 @@ __device__ __forceinline__ uint32_t slot_expert(const I* experts, uint32_t n, ui
     return id >= 0 && id < (I)num_experts ? (uint32_t)id : kDropped;
 }
 
-// counts[expert][block]
+// counts[expert * expert_step + block * block_step]
 template <typename I>
 __global__ __launch_bounds__(kRouteThreads) void route_count_kernel(const I* __restrict__ experts, uint32_t n, uint32_t num_experts,
-                                                                    uint32_t* __restrict__ counts, uint32_t blocks) {
+                                                                    uint32_t* __restrict__ counts, uint32_t expert_step, uint32_t block_step) {
     __shared__ uint32_t hist[SAR_MAX_EXPERTS];
     const uint32_t tid = threadIdx.x, block = blockIdx.x;
+    uint32_t key[kRouteStrips];
+#pragma unroll
+    for (uint32_t s = 0; s < kRouteStrips; ++s) key[s] = slot_expert(experts, n, block * kRouteBlock + s * kRouteThreads + tid, num_experts);
     if (tid < num_experts) hist[tid] = 0;
     __syncthreads();
 #pragma unroll
-    for (uint32_t s = 0; s < kRouteStrips; ++s) {
-        const uint32_t key = slot_expert(experts, n, block * kRouteBlock + s * kRouteThreads + tid, num_experts);
-        if (key != kDropped) atomicAdd(&hist[key], 1u);
-    }
+    for (uint32_t s = 0; s < kRouteStrips; ++s)
+        if (key[s] != kDropped) atomicAdd(&hist[key[s]], 1u);
     __syncthreads();
-    if (tid < num_experts) counts[(uint64_t)tid * blocks + block] = hist[tid];
+    if (tid < num_experts) counts[(uint64_t)tid * expert_step + (uint64_t)block * block_step] = hist[tid];
 }
 
 // One wave per expert: counts[expert][block] becomes the number of its slots in earlier blocks, totals[expert] all.
@@ -278,7 +282,14 @@ __global__ __launch_bounds__(kWave) void route_scan_kernel(uint32_t* __restrict_
     if (lane == 0) totals[blockIdx.x] = before;
 }
 
-template <typename I, uint32_t STRIPS, bool MANY>
+// Threads of one part of the sum over blocks: the experts, rounded up to whole waves and a divisor of the workgroup.
+__host__ __device__ inline uint32_t route_part(uint32_t num_experts) {
+    uint32_t part = kWave;
+    while (part < num_experts) part *= 2;
+    return part;
+}
+
+template <typename I, uint32_t STRIPS, int HOW>
 __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(const I* __restrict__ experts, uint32_t n, uint32_t num_experts,
                                                                     uint32_t key_bits, const uint32_t* __restrict__ counts,
                                                                     const uint32_t* __restrict__ totals, uint32_t blocks,
@@ -286,16 +297,37 @@ __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(const I* __r
                                                                     int32_t* __restrict__ offsets) {
     __shared__ uint16_t seen[kRouteWaves * SAR_MAX_EXPERTS];   // slots of an expert: this wave's so far, then earlier waves'
     __shared__ uint32_t first[SAR_MAX_EXPERTS];
+    __shared__ uint32_t part_before[HOW == kRouteSum ? kRouteThreads : 1], part_all[HOW == kRouteSum ? kRouteThreads : 1];
     __shared__ uint32_t wave_total[kRouteWaves];
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wave = uniform(tid / kWave);
     const uint32_t begin = blockIdx.x * (kRouteThreads * STRIPS);
     uint16_t* const mine = seen + wave * num_experts;
-    for (uint32_t i = lane; i < num_experts; i += kWave) mine[i] = 0;
 
     uint32_t key[STRIPS], place[STRIPS];
 #pragma unroll
     for (uint32_t s = 0; s < STRIPS; ++s)
         key[s] = slot_expert(experts, n, begin + (wave * STRIPS + s) * kWave + lane, num_experts);
+    uint32_t sum = 0, before = 0;                                // slots of expert `tid`: all, and in earlier blocks
+    if (HOW == kRouteScanned && tid < num_experts) {
+        sum = totals[tid];
+        before = counts[(uint64_t)tid * blocks + blockIdx.x];
+    }
+    const uint32_t part = HOW == kRouteSum ? route_part(num_experts) : 1u;
+    if (HOW == kRouteSum) {
+        const uint32_t expert = tid & (part - 1u), parts = kRouteThreads / part;
+        uint32_t early = 0, all = 0;
+        if (expert < num_experts) {
+#pragma unroll 8
+            for (uint32_t b = tid / part; b < blocks; b += parts) {
+                const uint32_t v = counts[(uint64_t)b * num_experts + expert];
+                all += v;
+                early += b < blockIdx.x ? v : 0u;
+            }
+        }
+        part_before[tid] = early;
+        part_all[tid] = all;
+    }
+    for (uint32_t i = lane; i < num_experts; i += kWave) mine[i] = 0;
     const uint64_t below = (1ull << lane) - 1ull;
 #pragma unroll
     for (uint32_t s = 0; s < STRIPS; ++s) {
@@ -315,14 +347,18 @@ __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(const I* __r
     }
     __syncthreads();
 
-    uint32_t sum = 0;                                            // this block's slots of expert `tid`
     if (tid < num_experts) {
+        uint32_t v[kRouteWaves], so_far = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kRouteWaves; ++w) v[w] = seen[w * num_experts + tid];
+#pragma unroll
         for (uint32_t w = 0; w < kRouteWaves; ++w) {
-            const uint32_t v = seen[w * num_experts + tid];
-            seen[w * num_experts + tid] = (uint16_t)sum;
-            sum += v;
+            seen[w * num_experts + tid] = (uint16_t)so_far;
+            so_far += v[w];
         }
-        if (MANY) sum = totals[tid];
+        if (HOW == kRouteAlone) sum = so_far;
+        if (HOW == kRouteSum)
+            for (uint32_t p = tid; p < kRouteThreads; p += part) { sum += part_all[p]; before += part_before[p]; }
     }
     uint32_t upto = sum;                                         // inclusive sum over the experts, wave by wave
     for (uint32_t d = 1; d < kWave; d <<= 1) {
@@ -337,7 +373,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(const I* __r
         total += wave_total[w];
     }
     if (tid < num_experts) {
-        first[tid] = upto - sum + (MANY ? counts[(uint64_t)tid * blocks + blockIdx.x] : 0u);
+        first[tid] = upto - sum + before;
         if (blockIdx.x == 0) offsets[tid] = (int32_t)(upto - sum);
     }
     if (blockIdx.x == 0 && tid == 0) offsets[num_experts] = (int32_t)total;
@@ -888,15 +924,26 @@ void launch_route(hipStream_t st, const void* experts, uint32_t n, uint32_t num_
     uint32_t bits = 0;
     while ((1u << bits) < num_experts) ++bits;
     if (n <= kRouteOne) {
-        route_place_kernel<I, kRouteOneStrips, false><<<1, kRouteThreads, 0, st>>>(ids, n, num_experts, bits, nullptr, nullptr, 1, row_of_slot, slot_of_row, offsets);
+        auto alone = [&](auto strips) {
+            route_place_kernel<I, decltype(strips)::value, kRouteAlone><<<1, kRouteThreads, 0, st>>>(ids, n, num_experts, bits, nullptr, nullptr, 1, row_of_slot, slot_of_row, offsets);
+        };
+        if (n <= kRouteThreads) alone(std::integral_constant<uint32_t, 1>{});
+        else if (n <= 4 * kRouteThreads) alone(std::integral_constant<uint32_t, 4>{});
+        else alone(std::integral_constant<uint32_t, kRouteOneStrips>{});
         return;
     }
     const uint32_t blocks = (uint32_t)route_blocks(n);
+    if (blocks * (uint64_t)route_part(num_experts) <= kRouteSumMost) {
+        uint32_t* const counts = workspace;
+        route_count_kernel<I><<<blocks, kRouteThreads, 0, st>>>(ids, n, num_experts, counts, 1, num_experts);
+        route_place_kernel<I, kRouteStrips, kRouteSum><<<blocks, kRouteThreads, 0, st>>>(ids, n, num_experts, bits, counts, nullptr, blocks, row_of_slot, slot_of_row, offsets);
+        return;
+    }
     uint32_t* const totals = workspace;
     uint32_t* const counts = workspace + num_experts;
-    route_count_kernel<I><<<blocks, kRouteThreads, 0, st>>>(ids, n, num_experts, counts, blocks);
+    route_count_kernel<I><<<blocks, kRouteThreads, 0, st>>>(ids, n, num_experts, counts, blocks, 1);
     route_scan_kernel<<<num_experts, kWave, 0, st>>>(counts, totals, blocks);
-    route_place_kernel<I, kRouteStrips, true><<<blocks, kRouteThreads, 0, st>>>(ids, n, num_experts, bits, counts, totals, blocks, row_of_slot, slot_of_row, offsets);
+    route_place_kernel<I, kRouteStrips, kRouteScanned><<<blocks, kRouteThreads, 0, st>>>(ids, n, num_experts, bits, counts, totals, blocks, row_of_slot, slot_of_row, offsets);
 }
 
 // What dispatch, combine and its backward pass have in common; null pointers that a call does not use are its own affair.
