@@ -195,9 +195,10 @@ __device__ __forceinline__ float wave_sum(float x) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), kWave - 1));
 }
 
-// Sums over a workgroup, in every lane.  `turn` alternates between two halves of the scratch, so that one barrier a
-// sum is enough: a half is written again only after everybody has passed the barrier of the sum in between.
-struct BlockSum {
+// Sums over the waves that share a row (all of the workgroup's, or `waves` consecutive ones of it), in every lane.
+// `turn` alternates between two halves of the scratch, so that one barrier a sum is enough: a half is written again only
+// after everybody has passed the barrier of the sum in between.  The whole workgroup takes part in every sum.
+struct RowSum {
     float* scratch;   // 2 * 2 * 16 floats of LDS
     uint32_t turn, waves, wave, lane;
     __device__ __forceinline__ void operator()(float& a, float& b) {
@@ -208,6 +209,7 @@ struct BlockSum {
         ++turn;
         if (lane == 0) { s[wave] = a; s[16 + wave] = b; }
         __syncthreads();
+        s += wave / waves * waves;
         a = b = 0.f;
         for (uint32_t w = 0; w < waves; ++w) { a += s[w]; b += s[16 + w]; }
     }
@@ -218,6 +220,7 @@ struct BlockSum {
         ++turn;
         if (lane == 0) s[wave] = a;
         __syncthreads();
+        s += wave / waves * waves;
         a = 0.f;
         for (uint32_t w = 0; w < waves; ++w) a += s[w];
     }
@@ -596,21 +599,24 @@ struct NormArgs {
 };
 
 constexpr uint32_t kNormThreads = 1024;
+constexpr uint32_t kRowsThreads = 512;   // backward pass: workgroups of short rows take several of them up to here
 
-// The V vectors of a thread: threadIdx.x, threadIdx.x + blockDim.x, ...
+// A thread's place in its row: it takes vectors at, at + step, ...
+struct RowPart { uint32_t at, step; };
+
 template <int DT, int VE, int V> struct Vectors { typename Raw<DT, VE>::T v[V]; };
 
 template <int DT, int VE, int V, bool NT = false>
-__device__ __forceinline__ Vectors<DT, VE, V> load_row(const char* row, const NormArgs& a) {
-    Vectors<DT, VE, V> r;
+__device__ __forceinline__ Vectors<DT, VE, V> load_row(const char* row, const NormArgs& a, RowPart r) {
+    Vectors<DT, VE, V> x;
 #pragma unroll
-    for (int v = 0; v < V; ++v) r.v[v] = load<DT, VE, NT>(row, Place<DT, VE>(threadIdx.x + v * blockDim.x, a.nvec, a.dim).byte());
-    return r;
+    for (int v = 0; v < V; ++v) x.v[v] = load<DT, VE, NT>(row, Place<DT, VE>(r.at + v * r.step, a.nvec, a.dim).byte());
+    return x;
 }
 template <int DT, int VE, int V>
-__device__ __forceinline__ void load_params(const char* p, bool f32, const NormArgs& a, float (&x)[V][VE]) {
+__device__ __forceinline__ void load_params(const char* p, bool f32, const NormArgs& a, RowPart r, float (&x)[V][VE]) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) load_param<DT, VE>(p, f32, Place<DT, VE>(threadIdx.x + v * blockDim.x, a.nvec, a.dim).elem, x[v]);
+    for (int v = 0; v < V; ++v) load_param<DT, VE>(p, f32, Place<DT, VE>(r.at + v * r.step, a.nvec, a.dim).elem, x[v]);
 }
 template <int V, int VE>
 __device__ __forceinline__ void set(float (&x)[V][VE], float value) {
@@ -631,24 +637,24 @@ __device__ __forceinline__ void add_row(float (&x)[V][VE], const Vectors<DT, VE,
 }
 // `count` copies of a row, `step` bytes apart
 template <int DT, int VE, int V, bool NT>
-__device__ __forceinline__ void store_row(char* to, uint64_t step, uint32_t count, const float (&x)[V][VE], const NormArgs& a) {
-    Vectors<DT, VE, V> r;
+__device__ __forceinline__ void store_row(char* to, uint64_t step, uint32_t count, const float (&x)[V][VE], const NormArgs& a, RowPart r) {
+    Vectors<DT, VE, V> out;
 #pragma unroll
-    for (int v = 0; v < V; ++v) r.v[v] = pack<DT, VE>(x[v]);
+    for (int v = 0; v < V; ++v) out.v[v] = pack<DT, VE>(x[v]);
     for (uint32_t c = 0; c < count; ++c, to += step) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const Place<DT, VE> p(threadIdx.x + v * blockDim.x, a.nvec, a.dim);
-            if (p.in) store<DT, VE, NT>(to, p.byte(), r.v[v]);
+            const Place<DT, VE> p(r.at + v * r.step, a.nvec, a.dim);
+            if (p.in) store<DT, VE, NT>(to, p.byte(), out.v[v]);
         }
     }
 }
 // a row in 32 bits, or in DT if f32 is false
 template <int DT, int VE, int V>
-__device__ __forceinline__ void store_params(char* to, bool f32, const float (&x)[V][VE], const NormArgs& a) {
+__device__ __forceinline__ void store_params(char* to, bool f32, const float (&x)[V][VE], const NormArgs& a, RowPart r) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const Place<DT, VE> p(threadIdx.x + v * blockDim.x, a.nvec, a.dim);
+        const Place<DT, VE> p(r.at + v * r.step, a.nvec, a.dim);
         if (!p.in) continue;
         if (DT == SAR_F32 || f32) {
             if constexpr (VE == 1) store<SAR_F32, 1>(to, p.elem * 4u, __float_as_uint(x[v][0]));
@@ -663,11 +669,11 @@ __device__ __forceinline__ void store_params(char* to, bool f32, const float (&x
 }
 // this thread's part of the sum over a row of x * y, doubled elements once
 template <int DT, int VE, int V>
-__device__ __forceinline__ float dot_row(const float (&x)[V][VE], const float (&y)[V][VE], const NormArgs& a) {
+__device__ __forceinline__ float dot_row(const float (&x)[V][VE], const float (&y)[V][VE], const NormArgs& a, RowPart r) {
     float s = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const Place<DT, VE> p(threadIdx.x + v * blockDim.x, a.nvec, a.dim);
+        const Place<DT, VE> p(r.at + v * r.step, a.nvec, a.dim);
 #pragma unroll
         for (int i = 0; i < VE; ++i) s = (uint32_t)i >= p.skip ? fmaf(x[v][i], y[v][i], s) : s;
     }
@@ -677,37 +683,37 @@ __device__ __forceinline__ float dot_row(const float (&x)[V][VE], const float (&
 template <int DT, int VE, int V, bool NT>
 __global__ __launch_bounds__(kNormThreads) void reduce_norm_kernel(const NormArgs a) {
     constexpr uint32_t ES = ElemSize<DT>::value;
-    constexpr bool KEEP = V * VE <= 8;      // weights stay in registers from token to token while that leaves room
+    constexpr bool kEarly = V * VE <= 8;    // weights for the first half are loaded beside the row where there are registers
     __shared__ float scratch[64];
-    BlockSum sum{scratch, 0u, blockDim.x / kWave, uniform(threadIdx.x / kWave), threadIdx.x & (kWave - 1)};
+    const RowPart r{threadIdx.x, blockDim.x};
+    RowSum sum{scratch, 0u, blockDim.x / kWave, uniform(threadIdx.x / kWave), threadIdx.x & (kWave - 1)};
     float post[V][VE], pre[V][VE], gate[V][VE];
-    if (KEEP) {
-        if (a.post) load_params<DT, VE, V>(a.post, a.post_f32, a, post);
-        if (a.pre) load_params<DT, VE, V>(a.pre, a.pre_f32, a, pre);
-        if (a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, gate);
-    }
     for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
         const uint64_t at = token * a.row_bytes;
-        const auto res = load_row<DT, VE, V, NT>(a.residual + at, a);
-        if (a.gate_kind == SAR_GATE_FULL) load_params<DT, VE, V>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, a, gate);
+        const auto res = load_row<DT, VE, V, NT>(a.residual + at, a, r);
+        if (kEarly) {
+            if (a.post) load_params<DT, VE, V>(a.post, a.post_f32, a, r, post);
+            if (a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, r, gate);
+        }
+        if (a.gate_kind == SAR_GATE_FULL) load_params<DT, VE, V>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, a, r, gate);
         if (a.gate_kind == SAR_GATE_TOKEN) set(gate, load_one<DT>(a.gate, a.gate_f32, token));
         float x[V][VE];
         set(x, 0.f);
-        in_batches<8 / V>(a.sources, [&](uint32_t s) { return load_row<DT, VE, V, NT>(a.partials[s] + at, a); },
-                   [&](const Vectors<DT, VE, V>& r) { add_row<DT, VE, V>(x, r); });
-        if (a.total) store_params<DT, VE, V>((char*)(a.total + token * a.dim), true, x, a);
+        in_batches<8 / V>(a.sources, [&](uint32_t s) { return load_row<DT, VE, V, NT>(a.partials[s] + at, a, r); },
+                   [&](const Vectors<DT, VE, V>& p) { add_row<DT, VE, V>(x, p); });
+        if (a.total) store_params<DT, VE, V>((char*)(a.total + token * a.dim), true, x, a, r);
         float r1 = 1.f;
         if (a.post) {
-            r1 = dot_row<DT, VE, V>(x, x, a);
+            r1 = dot_row<DT, VE, V>(x, x, a, r);
             sum(r1);
             r1 = rsqrtf(fmaf(r1, a.inv_dim, a.eps));
-            if (!KEEP) load_params<DT, VE, V>(a.post, a.post_f32, a, post);
+            if (!kEarly) load_params<DT, VE, V>(a.post, a.post_f32, a, r, post);
 #pragma unroll
             for (int v = 0; v < V; ++v)
 #pragma unroll
                 for (int i = 0; i < VE; ++i) x[v][i] = x[v][i] * r1 * post[v][i];
         }
-        if (!KEEP && a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, gate);
+        if (!kEarly && a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, r, gate);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float h[VE];
@@ -715,18 +721,18 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_kernel(const NormArg
 #pragma unroll
             for (int i = 0; i < VE; ++i) x[v][i] = fmaf(a.residual_scale, h[i], a.gate_kind == SAR_GATE_NONE ? x[v][i] : gate[v][i] * x[v][i]);
         }
-        if (a.hidden) store_row<DT, VE, V, NT>(a.hidden + at, 0, 1, x, a);
+        if (a.hidden) store_row<DT, VE, V, NT>(a.hidden + at, 0, 1, x, a, r);
         float r2 = 1.f;
         if (a.pre) {
-            r2 = dot_row<DT, VE, V>(x, x, a);
+            r2 = dot_row<DT, VE, V>(x, x, a, r);
             sum(r2);
             r2 = rsqrtf(fmaf(r2, a.inv_dim, a.eps));
-            if (!KEEP) load_params<DT, VE, V>(a.pre, a.pre_f32, a, pre);
+            load_params<DT, VE, V>(a.pre, a.pre_f32, a, r, pre);
 #pragma unroll
             for (int v = 0; v < V; ++v)
 #pragma unroll
                 for (int i = 0; i < VE; ++i) x[v][i] = x[v][i] * r2 * pre[v][i];
-            store_row<DT, VE, V, NT>(a.normed + at, a.copy_bytes, a.copies, x, a);
+            store_row<DT, VE, V, NT>(a.normed + at, a.copy_bytes, a.copies, x, a, r);
         }
         if (a.stats && threadIdx.x == 0) { a.stats[token] = r1; a.stats[a.tokens + token] = r2; }
     }
@@ -749,35 +755,42 @@ struct NormBackwardArgs {
     char* grad_gate;                   // per token or full (a channel gate's gradient is a column sum)
     float* columns;                    // [workgroup][3][dim]
     uint32_t total_f32, want_pre, want_post, want_gate;   // want_gate: a channel gate's
+    uint32_t row_threads;              // threads of one row
 };
 
 template <int DT, int VE, int V, bool NT>
 __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(const NormBackwardArgs b) {
     constexpr uint32_t ES = ElemSize<DT>::value;
+    constexpr uint32_t kMost = V == 1 ? kRowsThreads : 0u;              // threads of a workgroup that takes several tokens
     __shared__ float scratch[64];
+    __shared__ float rows[kMost ? kMost * VE : 1];
     const NormArgs& a = b.f;
-    BlockSum sum{scratch, 0u, blockDim.x / kWave, uniform(threadIdx.x / kWave), threadIdx.x & (kWave - 1)};
+    const uint32_t many = blockDim.x / b.row_threads, mine = many == 1 ? 0u : uniform(threadIdx.x / b.row_threads);
+    const RowPart r{threadIdx.x - mine * b.row_threads, b.row_threads};
+    RowSum sum{scratch, 0u, b.row_threads / kWave, uniform(threadIdx.x / kWave), threadIdx.x & (kWave - 1)};
     float col_pre[V][VE], col_post[V][VE], col_gate[V][VE];
     set(col_pre, 0.f), set(col_post, 0.f), set(col_gate, 0.f);
-    for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
+    for (uint64_t first = (uint64_t)blockIdx.x * many; first < a.tokens; first += (uint64_t)gridDim.x * many) {
+        const bool in = first + mine < a.tokens;                        // the sums are the whole workgroup's affair
+        const uint64_t token = in ? first + mine : a.tokens - 1;
         const uint64_t at = token * a.row_bytes;
         const float r1 = a.stats[token], r2 = a.stats[a.tokens + token];
         const float token_gate = a.gate_kind == SAR_GATE_TOKEN ? load_one<DT>(a.gate, a.gate_f32, token) : 1.f;
-        const auto res = load_row<DT, VE, V, NT>(a.residual + at, a);
+        const auto res = load_row<DT, VE, V, NT>(a.residual + at, a, r);
         Vectors<DT, VE, V> gh{};
-        if (b.grad_hidden) gh = load_row<DT, VE, V, NT>(b.grad_hidden + at, a);
+        if (b.grad_hidden) gh = load_row<DT, VE, V, NT>(b.grad_hidden + at, a, r);
         float y[V][VE];      // yhat (y without a norm there)
-        load_params<DT, VE, V>(b.total + token * a.dim * (b.total_f32 ? 4u : ES), b.total_f32, a, y);
+        load_params<DT, VE, V>(b.total + token * a.dim * (b.total_f32 ? 4u : ES), b.total_f32, a, r, y);
         float d[V][VE];      // G, then G pre, then d hidden
         set(d, 0.f);
         if (b.grad_normed)
-            in_batches<V == 1 ? 4 : 8 / V>(a.copies, [&](uint32_t c) { return load_row<DT, VE, V, NT>(b.grad_normed + at + c * a.copy_bytes, a); },
-                       [&](const Vectors<DT, VE, V>& r) { add_row<DT, VE, V>(d, r); });
+            in_batches<V == 1 ? 4 : 8 / V>(a.copies, [&](uint32_t c) { return load_row<DT, VE, V, NT>(b.grad_normed + at + c * a.copy_bytes, a, r); },
+                       [&](const Vectors<DT, VE, V>& p) { add_row<DT, VE, V>(d, p); });
         float post[V][VE], gate[V][VE], h[V][VE];      // h: hhat
-        if (a.post) load_params<DT, VE, V>(a.post, a.post_f32, a, post);
+        if (a.post) load_params<DT, VE, V>(a.post, a.post_f32, a, r, post);
         else set(post, 1.f);
-        if (a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, gate);
-        else if (a.gate_kind == SAR_GATE_FULL) load_params<DT, VE, V>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, a, gate);
+        if (a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, r, gate);
+        else if (a.gate_kind == SAR_GATE_FULL) load_params<DT, VE, V>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, a, r, gate);
         else set(gate, token_gate);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -790,15 +803,15 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
         }
         if (b.grad_normed) {
             float pre[V][VE];
-            load_params<DT, VE, V>(a.pre, a.pre_f32, a, pre);
+            load_params<DT, VE, V>(a.pre, a.pre_f32, a, r, pre);
 #pragma unroll
             for (int v = 0; v < V; ++v)
 #pragma unroll
                 for (int i = 0; i < VE; ++i) {
-                    col_pre[v][i] = fmaf(d[v][i], h[v][i], col_pre[v][i]);
+                    if (in) col_pre[v][i] = fmaf(d[v][i], h[v][i], col_pre[v][i]);
                     d[v][i] *= pre[v][i];
                 }
-            float mean = dot_row<DT, VE, V>(d, h, a);
+            float mean = dot_row<DT, VE, V>(d, h, a, r);
             sum(mean);
             mean *= a.inv_dim;
 #pragma unroll
@@ -807,30 +820,32 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
                 for (int i = 0; i < VE; ++i) d[v][i] = r2 * fmaf(-h[v][i], mean, d[v][i]);
         }
         if (b.grad_hidden) add_row<DT, VE, V>(d, gh);
-        if (b.grad_residual) {
+        if (b.grad_residual && in) {
 #pragma unroll
             for (int v = 0; v < V; ++v)
 #pragma unroll
                 for (int i = 0; i < VE; ++i) h[v][i] = a.residual_scale * d[v][i];
-            store_row<DT, VE, V, NT>(b.grad_residual + at, 0, 1, h, a);
+            store_row<DT, VE, V, NT>(b.grad_residual + at, 0, 1, h, a, r);
         }
         float gate_dot = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const Place<DT, VE> p(threadIdx.x + v * blockDim.x, a.nvec, a.dim);
+            const Place<DT, VE> p(r.at + v * r.step, a.nvec, a.dim);
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
                 const float du = d[v][i] * gate[v][i];
                 h[v][i] = d[v][i] * (y[v][i] * post[v][i]);                  // gradient of the gate
-                col_gate[v][i] += h[v][i];
-                col_post[v][i] = fmaf(du, y[v][i], col_post[v][i]);
+                if (in) {
+                    col_gate[v][i] += h[v][i];
+                    col_post[v][i] = fmaf(du, y[v][i], col_post[v][i]);
+                }
                 d[v][i] = du * post[v][i];
                 gate_dot += (uint32_t)i >= p.skip ? h[v][i] : 0.f;
             }
         }
-        if (a.gate_kind == SAR_GATE_FULL && b.grad_gate) store_params<DT, VE, V>(b.grad_gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, h, a);
+        if (a.gate_kind == SAR_GATE_FULL && b.grad_gate && in) store_params<DT, VE, V>(b.grad_gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, h, a, r);
         if (a.post) {
-            float mean = dot_row<DT, VE, V>(d, y, a);
+            float mean = dot_row<DT, VE, V>(d, y, a, r);
             sum(mean, gate_dot);
             mean *= a.inv_dim;
 #pragma unroll
@@ -840,16 +855,31 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
         } else if (a.gate_kind == SAR_GATE_TOKEN) {
             sum(gate_dot);
         }
-        if (a.gate_kind == SAR_GATE_TOKEN && b.grad_gate && threadIdx.x == 0) store_one<DT>(b.grad_gate, a.gate_f32, token, gate_dot);
-        if (b.grad_partials) store_row<DT, VE, V, NT>(b.grad_partials + at, a.copy_bytes, a.sources, d, a);
+        if (a.gate_kind == SAR_GATE_TOKEN && b.grad_gate && in && r.at == 0) store_one<DT>(b.grad_gate, a.gate_f32, token, gate_dot);
+        if (b.grad_partials && in) store_row<DT, VE, V, NT>(b.grad_partials + at, a.copy_bytes, a.sources, d, a, r);
     }
-    char* const columns = (char*)(b.columns + (uint64_t)blockIdx.x * 3u * a.dim);
-    if (b.want_pre) store_params<DT, VE, V>(columns, true, col_pre, a);
-    if (b.want_post) store_params<DT, VE, V>(columns + (uint64_t)a.dim * 4u, true, col_post, a);
-    if (b.want_gate) store_params<DT, VE, V>(columns + (uint64_t)a.dim * 8u, true, col_gate, a);
+    auto leave = [&](float (&x)[V][VE], uint32_t which) {
+        if constexpr (kMost != 0u) {
+            if (many > 1) {                                              // the rows' sums, in their order
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < VE; ++i) rows[threadIdx.x * VE + i] = x[0][i];
+                __syncthreads();
+                if (mine) return;
+                for (uint32_t m = 1; m < many; ++m)
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) x[0][i] += rows[(m * r.step + r.at) * VE + i];
+            }
+        }
+        store_params<DT, VE, V>((char*)(b.columns + ((uint64_t)blockIdx.x * 3u + which) * a.dim), true, x, a, r);
+    };
+    if (b.want_pre) leave(col_pre, 0);
+    if (b.want_post) leave(col_post, 1);
+    if (b.want_gate) leave(col_gate, 2);
 }
 
-// Adds the workgroups' rows of column sums: 64 columns a workgroup, 16 waves taking every 16th row, then in wave order.
+// Adds the workgroups' rows of column sums: 32 columns a workgroup, 32 groups of threads taking every 32nd row, then in
+// the groups' order.
 struct ColumnArgs {
     const float* columns;
     char* out[3];
@@ -858,18 +888,22 @@ struct ColumnArgs {
 };
 template <int DT>
 __global__ __launch_bounds__(1024) void column_sum_kernel(const ColumnArgs a) {
-    __shared__ float part[16][kWave];
-    const uint32_t which = blockIdx.y, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    __shared__ float part[32][33];
+    const uint32_t which = blockIdx.y, lane = threadIdx.x & 31u, group = threadIdx.x / 32u;
     if (!a.out[which]) return;
-    const uint32_t col = blockIdx.x * kWave + lane;
+    const uint32_t col = blockIdx.x * 32u + lane;
     float s = 0.f;
-    if (col < a.dim)
-        for (uint32_t r = wave; r < a.rows; r += 16) s += a.columns[((uint64_t)r * 3u + which) * a.dim + col];
-    part[wave][lane] = s;
+    if (col < a.dim) {
+        const float* from = a.columns + which * a.dim + col;
+#pragma unroll 8
+        for (uint32_t r = group; r < a.rows; r += 32u) s += from[(uint64_t)r * 3u * a.dim];
+    }
+    part[group][lane] = s;
     __syncthreads();
-    if (wave == 0 && col < a.dim) {
+    if (group == 0 && col < a.dim) {
         s = 0.f;
-        for (int w = 0; w < 16; ++w) s += part[w][lane];
+#pragma unroll
+        for (int g = 0; g < 32; ++g) s += part[g][lane];
         store_one<DT>(a.out[which], a.f32[which], col, s);
     }
 }
@@ -1049,12 +1083,16 @@ NormShape norm_shape(int dtype, int64_t dim) {
     return {threads, v, false};
 }
 
-// Workgroups of the backward pass: as many as the chip holds at once, with a few tokens for each so that the column
-// sums are a small part of the traffic.
+// Tokens a workgroup of the backward pass has in hand.
+uint32_t norm_backward_rows(const NormShape& s) { return s.vectors > 1 || s.threads > kRowsThreads ? 1u : kRowsThreads / s.threads; }
+
+// Workgroups of the backward pass: as many as the chip holds at once (a token for each row of threads is enough: 8 tokens
+// of 4096 take 9.6 us so, 13.1 with two tokens in turn and fewer column sums, 20.3 with four; 1537 of 1001 15.0, 15.2, 19.4).
 uint32_t norm_backward_groups(int64_t tokens, int64_t dim, int dtype) {
-    const uint32_t waves = norm_shape(dtype, dim).threads / kWave;
-    const uint64_t resident = 256u * std::max(1u, std::min(4u, 16u / waves));
-    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(resident, ((uint64_t)tokens + 3) / 4));
+    const NormShape s = norm_shape(dtype, dim);
+    const uint32_t rows = norm_backward_rows(s);
+    const uint64_t resident = 256u * std::max(1u, 1024u / (s.threads * rows));
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(resident, ((uint64_t)tokens + rows - 1) / rows));
 }
 
 const char* check_norm(const sar_reduce_norm_args* a) {
@@ -1128,7 +1166,7 @@ template <int DT> void launch_norm_backward(hipStream_t st, const NormBackwardAr
     const NormArgs& a = b.f;
     const uint64_t rows = (b.grad_partials ? a.sources : 0) + 3 + (b.grad_normed ? a.copies : 0) + (b.total_f32 ? 4 / ElemSize<DT>::value : 1);
     with_bool(rows * a.copy_bytes >= kStreamBytes, [&](auto nt) {
-        with_norm_shape<DT>(s, [&](auto ve, auto v) { reduce_norm_backward_kernel<DT, decltype(ve)::value, decltype(v)::value, decltype(nt)::value><<<grid, s.threads, 0, st>>>(b); });
+        with_norm_shape<DT>(s, [&](auto ve, auto v) { reduce_norm_backward_kernel<DT, decltype(ve)::value, decltype(v)::value, decltype(nt)::value><<<grid, s.threads * norm_backward_rows(s), 0, st>>>(b); });
     });
 }
 
@@ -1291,6 +1329,7 @@ int sar_reduce_norm_backward(int device, void* stream, const sar_reduce_norm_arg
         b.want_gate = channel && g->grad_gate != nullptr;
         const uint32_t groups = norm_backward_groups(forward->tokens, forward->dim, forward->dtype);
         const NormShape shape = norm_shape(forward->dtype, forward->dim);
+        b.row_threads = shape.threads;
         with_dtype(forward->dtype, [&](auto dt) { launch_norm_backward<decltype(dt)::value>((hipStream_t)stream, b, shape, groups); });
         if (int rc = launched("sar_reduce_norm_backward")) return rc;
         if (b.want_pre || b.want_post || b.want_gate) {
@@ -1304,7 +1343,7 @@ int sar_reduce_norm_backward(int device, void* stream, const sar_reduce_norm_arg
             c.f32[2] = b.f.gate_f32;
             c.rows = groups;
             c.dim = b.f.dim;
-            const dim3 grid((c.dim + kWave - 1) / kWave, 3);
+            const dim3 grid((c.dim + 31u) / 32u, 3);
             with_dtype(forward->dtype, [&](auto dt) { column_sum_kernel<decltype(dt)::value><<<grid, 1024, 0, (hipStream_t)stream>>>(c); });
             return launched("sar_reduce_norm_backward");
         }
