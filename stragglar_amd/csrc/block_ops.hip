@@ -563,7 +563,7 @@ __global__ __launch_bounds__(kMoveThreads) void combine_backward_kernel(const Mo
                     s = wave_sum(s);
                     if ((int)lane == r.k) dot += s;
                 };
-                in_batches<4>(count, ld, use);
+                in_batches<2>(count, ld, use);
                 if (a.out) zero_rows<DT, VE, U, NT>(a, token, v0);
             }
             if (SHARE > 1) dots[wave][lane] = dot;
@@ -1056,8 +1056,12 @@ template <int DT> void launch_combine(hipStream_t st, const MoveArgs& a) {
     else combine_kernel<DT, kVec<DT>, U, false><<<move_grid(a, U), kMoveThreads, 0, st>>>(a);
 }
 
+// A wave takes a token, with as many vectors a lane as the row has; four waves share one where the row is longer than
+// that, or where there are too few tokens to keep the chip busy (32 tokens of 2048, eight choices: 5.4 us shared, 7.3 not;
+// 4099 of 1001, two choices: 13.3 shared, 11.7 not).  Two rows at a time: four cost registers and with them waves (50000
+// tokens of 256, one choice: 36.7 us against 46.1).
 template <int DT> void launch_combine_backward(hipStream_t st, const MoveArgs& a) {
-    const bool shared = a.nvec > 4 * kWave;
+    const bool shared = a.nvec > 4 * kWave || (a.nvec > kWave && a.tokens < 2048);
     const uint64_t groups = shared ? a.tokens : (a.tokens + kMoveWaves - 1) / kMoveWaves;
     const uint32_t grid = (uint32_t)std::min<uint64_t>(groups, 1u << 20);
     const bool nt = ((uint64_t)a.nrows * (a.out ? 2 : 1) + a.tokens) * a.row_bytes >= kStreamBytes;
@@ -1068,6 +1072,8 @@ template <int DT> void launch_combine_backward(hipStream_t st, const MoveArgs& a
     with_bool(nt, [&](auto stream) {
         constexpr bool NT = decltype(stream)::value;
         if (shared) combine_backward_kernel<DT, kVec<DT>, 2, 4, NT><<<grid, kMoveThreads, 0, st>>>(a);
+        else if (a.nvec <= kWave) combine_backward_kernel<DT, kVec<DT>, 1, 1, NT><<<grid, kMoveThreads, 0, st>>>(a);
+        else if (a.nvec <= 2 * kWave) combine_backward_kernel<DT, kVec<DT>, 2, 1, NT><<<grid, kMoveThreads, 0, st>>>(a);
         else combine_backward_kernel<DT, kVec<DT>, 4, 1, NT><<<grid, kMoveThreads, 0, st>>>(a);
     });
 }
