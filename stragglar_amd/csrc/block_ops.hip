@@ -23,6 +23,7 @@ namespace sar {
 namespace {
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
 typedef u4 u4_any __attribute__((aligned(2)));   // 16 bytes at any element boundary
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -758,6 +759,49 @@ struct NormBackwardArgs {
     uint32_t row_threads;              // threads of one row
 };
 
+// A thread's column sums, in registers or, for rows that leave none, in LDS (a thread touches its own only).
+template <int V, int VE, bool LDS> struct Columns {
+    float x[V][VE];
+    __device__ __forceinline__ void init(f4*) { set(x, 0.f); }
+    __device__ __forceinline__ void add(int v, const float (&a)[VE], const float (&b)[VE]) {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) x[v][i] = fmaf(a[i], b[i], x[v][i]);
+    }
+    __device__ __forceinline__ void get(float (&y)[V][VE]) const {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int i = 0; i < VE; ++i) y[v][i] = x[v][i];
+    }
+};
+template <int V, int VE> struct Columns<V, VE, true> {
+    f4* mine;          // entry of this thread; the next vector of four is kNormThreads further on
+    __device__ __forceinline__ void init(f4* lds) {
+        mine = lds + threadIdx.x;
+#pragma unroll
+        for (int q = 0; q < V * VE / 4; ++q) mine[q * kNormThreads] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void add(int v, const float (&a)[VE], const float (&b)[VE]) {
+#pragma unroll
+        for (int q = 0; q < VE / 4; ++q) {
+            f4 m = mine[(v * (VE / 4) + q) * kNormThreads];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m[i] = fmaf(a[4 * q + i], b[4 * q + i], m[i]);
+            mine[(v * (VE / 4) + q) * kNormThreads] = m;
+        }
+    }
+    __device__ __forceinline__ void get(float (&y)[V][VE]) const {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int q = 0; q < VE / 4; ++q) {
+                const f4 m = mine[(v * (VE / 4) + q) * kNormThreads];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[v][4 * q + i] = m[i];
+            }
+    }
+};
+
 template <int DT, int VE, int V, bool NT>
 __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(const NormBackwardArgs b) {
     constexpr uint32_t ES = ElemSize<DT>::value;
@@ -768,8 +812,12 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
     const uint32_t many = blockDim.x / b.row_threads, mine = many == 1 ? 0u : uniform(threadIdx.x / b.row_threads);
     const RowPart r{threadIdx.x - mine * b.row_threads, b.row_threads};
     RowSum sum{scratch, 0u, b.row_threads / kWave, uniform(threadIdx.x / kWave), threadIdx.x & (kWave - 1)};
-    float col_pre[V][VE], col_post[V][VE], col_gate[V][VE];
-    set(col_pre, 0.f), set(col_post, 0.f), set(col_gate, 0.f);
+    // 16 elements a thread: two of the three column sums (128 KB) stay in LDS, or 48 registers more would be spilled
+    constexpr bool kInLds = V * VE > 8;
+    __shared__ f4 lds[kInLds ? 2 * (V * VE / 4) * kNormThreads : 1];
+    Columns<V, VE, kInLds> col_pre, col_post;
+    Columns<V, VE, false> col_gate;
+    col_pre.init(lds), col_post.init(lds + (kInLds ? V * VE / 4 * kNormThreads : 0)), col_gate.init(nullptr);
     for (uint64_t first = (uint64_t)blockIdx.x * many; first < a.tokens; first += (uint64_t)gridDim.x * many) {
         const bool in = first + mine < a.tokens;                        // the sums are the whole workgroup's affair
         const uint64_t token = in ? first + mine : a.tokens - 1;
@@ -784,14 +832,17 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
         float d[V][VE];      // G, then G pre, then d hidden
         set(d, 0.f);
         if (b.grad_normed)
-            in_batches<V == 1 ? 4 : 8 / V>(a.copies, [&](uint32_t c) { return load_row<DT, VE, V, NT>(b.grad_normed + at + c * a.copy_bytes, a, r); },
+            in_batches<kInLds ? 8 / V / 2 : V == 1 ? 4 : 8 / V>(a.copies, [&](uint32_t c) { return load_row<DT, VE, V, NT>(b.grad_normed + at + c * a.copy_bytes, a, r); },
                        [&](const Vectors<DT, VE, V>& p) { add_row<DT, VE, V>(d, p); });
         float post[V][VE], gate[V][VE], h[V][VE];      // h: hhat
-        if (a.post) load_params<DT, VE, V>(a.post, a.post_f32, a, r, post);
-        else set(post, 1.f);
-        if (a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, r, gate);
-        else if (a.gate_kind == SAR_GATE_FULL) load_params<DT, VE, V>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, a, r, gate);
-        else set(gate, token_gate);
+        auto load_gates = [&]() {
+            if (a.post) load_params<DT, VE, V>(a.post, a.post_f32, a, r, post);
+            else set(post, 1.f);
+            if (a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, r, gate);
+            else if (a.gate_kind == SAR_GATE_FULL) load_params<DT, VE, V>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, a, r, gate);
+            else set(gate, token_gate);
+        };
+        load_gates();
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             unpack<DT, VE>(res.v[v], h[v]);
@@ -805,12 +856,11 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
             float pre[V][VE];
             load_params<DT, VE, V>(a.pre, a.pre_f32, a, r, pre);
 #pragma unroll
-            for (int v = 0; v < V; ++v)
+            for (int v = 0; v < V; ++v) {
+                if (in) col_pre.add(v, d[v], h[v]);
 #pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    if (in) col_pre[v][i] = fmaf(d[v][i], h[v][i], col_pre[v][i]);
-                    d[v][i] *= pre[v][i];
-                }
+                for (int i = 0; i < VE; ++i) d[v][i] *= pre[v][i];
+            }
             float mean = dot_row<DT, VE, V>(d, h, a, r);
             sum(mean);
             mean *= a.inv_dim;
@@ -828,20 +878,22 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
             store_row<DT, VE, V, NT>(b.grad_residual + at, 0, 1, h, a, r);
         }
         float gate_dot = 0.f;
+        if (kInLds) load_gates();                      // again, from the cache: kept they would be spilled
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const Place<DT, VE> p(r.at + v * r.step, a.nvec, a.dim);
 #pragma unroll
+            for (int i = 0; i < VE; ++i) h[v][i] = y[v][i] * post[v][i];       // u
+            if (in) col_gate.add(v, d[v], h[v]);
+#pragma unroll
             for (int i = 0; i < VE; ++i) {
-                const float du = d[v][i] * gate[v][i];
-                h[v][i] = d[v][i] * (y[v][i] * post[v][i]);                  // gradient of the gate
-                if (in) {
-                    col_gate[v][i] += h[v][i];
-                    col_post[v][i] = fmaf(du, y[v][i], col_post[v][i]);
-                }
-                d[v][i] = du * post[v][i];
+                h[v][i] *= d[v][i];                                          // gradient of the gate
                 gate_dot += (uint32_t)i >= p.skip ? h[v][i] : 0.f;
+                d[v][i] *= gate[v][i];
             }
+            if (in) col_post.add(v, d[v], y[v]);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) d[v][i] *= post[v][i];
         }
         if (a.gate_kind == SAR_GATE_FULL && b.grad_gate && in) store_params<DT, VE, V>(b.grad_gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, h, a, r);
         if (a.post) {
@@ -858,7 +910,9 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
         if (a.gate_kind == SAR_GATE_TOKEN && b.grad_gate && in && r.at == 0) store_one<DT>(b.grad_gate, a.gate_f32, token, gate_dot);
         if (b.grad_partials && in) store_row<DT, VE, V, NT>(b.grad_partials + at, a.copy_bytes, a.sources, d, a, r);
     }
-    auto leave = [&](float (&x)[V][VE], uint32_t which) {
+    auto leave = [&](const auto& columns, uint32_t which) {
+        float x[V][VE];
+        columns.get(x);
         if constexpr (kMost != 0u) {
             if (many > 1) {                                              // the rows' sums, in their order
                 __syncthreads();
