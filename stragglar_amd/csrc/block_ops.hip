@@ -95,7 +95,7 @@ __device__ __forceinline__ void in_batches(uint32_t count, Load&& ld, Use&& use)
     for (; s + MOST <= count; s += MOST) batch<MOST>(s, ld, use);
     if constexpr (MOST > 4) if (s + 4 <= count) { batch<4>(s, ld, use); s += 4; }
     if constexpr (MOST > 2) if (s + 2 <= count) { batch<2>(s, ld, use); s += 2; }
-    if (s < count) batch<1>(s, ld, use);
+    if constexpr (MOST > 1) if (s < count) batch<1>(s, ld, use);
 }
 
 __device__ __forceinline__ float widen(uint32_t bits, int dt) {   // one 16-bit element in the low half
@@ -626,6 +626,13 @@ __device__ __forceinline__ void set(float (&x)[V][VE], float value) {
 #pragma unroll
         for (int i = 0; i < VE; ++i) x[v][i] = value;
 }
+template <int V, int VE>
+__device__ __forceinline__ void copy(float (&x)[V][VE], const float (&y)[V][VE]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) x[v][i] = y[v][i];
+}
 template <int DT, int VE, int V>
 __device__ __forceinline__ void add_row(float (&x)[V][VE], const Vectors<DT, VE, V>& r) {
 #pragma unroll
@@ -681,7 +688,7 @@ __device__ __forceinline__ float dot_row(const float (&x)[V][VE], const float (&
     return s;
 }
 
-template <int DT, int VE, int V, bool NT>
+template <int DT, int VE, int V, bool ONE, bool NT>
 __global__ __launch_bounds__(kNormThreads) void reduce_norm_kernel(const NormArgs a) {
     constexpr uint32_t ES = ElemSize<DT>::value;
     constexpr bool kEarly = V * VE <= 8;    // weights for the first half are loaded beside the row where there are registers
@@ -700,8 +707,8 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_kernel(const NormArg
         if (a.gate_kind == SAR_GATE_TOKEN) set(gate, load_one<DT>(a.gate, a.gate_f32, token));
         float x[V][VE];
         set(x, 0.f);
-        in_batches<8 / V>(a.sources, [&](uint32_t s) { return load_row<DT, VE, V, NT>(a.partials[s] + at, a, r); },
-                   [&](const Vectors<DT, VE, V>& p) { add_row<DT, VE, V>(x, p); });
+        in_batches<ONE ? 1 : 8 / V>(ONE ? 1u : a.sources, [&](uint32_t s) { return load_row<DT, VE, V, NT>(a.partials[s] + at, a, r); },
+                                    [&](const Vectors<DT, VE, V>& p) { add_row<DT, VE, V>(x, p); });
         if (a.total) store_params<DT, VE, V>((char*)(a.total + token * a.dim), true, x, a, r);
         float r1 = 1.f;
         if (a.post) {
@@ -802,7 +809,7 @@ template <int V, int VE> struct Columns<V, VE, true> {
     }
 };
 
-template <int DT, int VE, int V, bool NT>
+template <int DT, int VE, int V, bool ONE, bool NT>
 __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(const NormBackwardArgs b) {
     constexpr uint32_t ES = ElemSize<DT>::value;
     constexpr uint32_t kMost = V == 1 ? kRowsThreads : 0u;              // threads of a workgroup that takes several tokens
@@ -818,6 +825,17 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
     Columns<V, VE, kInLds> col_pre, col_post;
     Columns<V, VE, false> col_gate;
     col_pre.init(lds), col_post.init(lds + (kInLds ? V * VE / 4 * kNormThreads : 0)), col_gate.init(nullptr);
+    // One row in, one row out: nothing to batch, so the weights stay in registers from token to token (4096 tokens of 4096
+    // 62 -> 50 us).  With eight rows to write it was slower so (20000 of 2048: 219 us against 240).
+    constexpr bool kKeep = ONE;
+    constexpr int kKept = kKeep ? V : 1, kKeptVE = kKeep ? VE : 1;
+    float kept_pre[kKept][kKeptVE], kept_post[kKept][kKeptVE], kept_gate[kKept][kKeptVE];
+    if constexpr (kKeep) {
+        if (a.pre) load_params<DT, VE, V>(a.pre, a.pre_f32, a, r, kept_pre);
+        if (a.post) load_params<DT, VE, V>(a.post, a.post_f32, a, r, kept_post);
+        else set(kept_post, 1.f);
+        if (a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, r, kept_gate);
+    }
     for (uint64_t first = (uint64_t)blockIdx.x * many; first < a.tokens; first += (uint64_t)gridDim.x * many) {
         const bool in = first + mine < a.tokens;                        // the sums are the whole workgroup's affair
         const uint64_t token = in ? first + mine : a.tokens - 1;
@@ -832,15 +850,21 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
         float d[V][VE];      // G, then G pre, then d hidden
         set(d, 0.f);
         if (b.grad_normed)
-            in_batches<kInLds ? 8 / V / 2 : V == 1 ? 4 : 8 / V>(a.copies, [&](uint32_t c) { return load_row<DT, VE, V, NT>(b.grad_normed + at + c * a.copy_bytes, a, r); },
+            in_batches<ONE ? 1 : kInLds ? 8 / V / 2 : V == 1 ? 4 : 8 / V>(ONE ? 1u : a.copies, [&](uint32_t c) { return load_row<DT, VE, V, NT>(b.grad_normed + at + c * a.copy_bytes, a, r); },
                        [&](const Vectors<DT, VE, V>& p) { add_row<DT, VE, V>(d, p); });
         float post[V][VE], gate[V][VE], h[V][VE];      // h: hhat
         auto load_gates = [&]() {
-            if (a.post) load_params<DT, VE, V>(a.post, a.post_f32, a, r, post);
+            if constexpr (kKeep) copy(post, kept_post);
+            else if (a.post) load_params<DT, VE, V>(a.post, a.post_f32, a, r, post);
             else set(post, 1.f);
-            if (a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, r, gate);
-            else if (a.gate_kind == SAR_GATE_FULL) load_params<DT, VE, V>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, a, r, gate);
-            else set(gate, token_gate);
+            if (a.gate_kind == SAR_GATE_CHANNEL) {
+                if constexpr (kKeep) copy(gate, kept_gate);
+                else load_params<DT, VE, V>(a.gate, a.gate_f32, a, r, gate);
+            } else if (a.gate_kind == SAR_GATE_FULL) {
+                load_params<DT, VE, V>(a.gate + token * a.dim * (a.gate_f32 ? 4u : ES), a.gate_f32, a, r, gate);
+            } else {
+                set(gate, token_gate);
+            }
         };
         load_gates();
 #pragma unroll
@@ -854,7 +878,8 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
         }
         if (b.grad_normed) {
             float pre[V][VE];
-            load_params<DT, VE, V>(a.pre, a.pre_f32, a, r, pre);
+            if constexpr (kKeep) copy(pre, kept_pre);
+            else load_params<DT, VE, V>(a.pre, a.pre_f32, a, r, pre);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 if (in) col_pre.add(v, d[v], h[v]);
@@ -1218,7 +1243,10 @@ template <int DT> void launch_norm(hipStream_t st, const NormArgs& a, const Norm
     const uint32_t grid = (uint32_t)std::min<uint64_t>(a.tokens, 1u << 20);
     const uint64_t rows = a.sources + 2 + (a.normed ? a.copies : 0) + (a.total ? 4 / ElemSize<DT>::value : 0);
     with_bool(rows * a.copy_bytes >= kStreamBytes, [&](auto nt) {
-        with_norm_shape<DT>(s, [&](auto ve, auto v) { reduce_norm_kernel<DT, decltype(ve)::value, decltype(v)::value, decltype(nt)::value><<<grid, s.threads, 0, st>>>(a); });
+        // a finished output asks for no batch of rows: fewer registers, more rows in flight (4096 of 4096: 30.1 -> 25.9 us)
+        with_bool(a.sources == 1, [&](auto one) {
+            with_norm_shape<DT>(s, [&](auto ve, auto v) { reduce_norm_kernel<DT, decltype(ve)::value, decltype(v)::value, decltype(one)::value, decltype(nt)::value><<<grid, s.threads, 0, st>>>(a); });
+        });
     });
 }
 
@@ -1226,7 +1254,13 @@ template <int DT> void launch_norm_backward(hipStream_t st, const NormBackwardAr
     const NormArgs& a = b.f;
     const uint64_t rows = (b.grad_partials ? a.sources : 0) + 3 + (b.grad_normed ? a.copies : 0) + (b.total_f32 ? 4 / ElemSize<DT>::value : 1);
     with_bool(rows * a.copy_bytes >= kStreamBytes, [&](auto nt) {
-        with_norm_shape<DT>(s, [&](auto ve, auto v) { reduce_norm_backward_kernel<DT, decltype(ve)::value, decltype(v)::value, decltype(nt)::value><<<grid, s.threads * norm_backward_rows(s), 0, st>>>(b); });
+        with_bool(a.sources == 1 && a.copies == 1, [&](auto one) {
+            with_norm_shape<DT>(s, [&](auto ve, auto v) {
+                constexpr int VE = decltype(ve)::value, V = decltype(v)::value;
+                constexpr bool ONE = decltype(one)::value && V == 1;
+                reduce_norm_backward_kernel<DT, VE, V, ONE, decltype(nt)::value><<<grid, s.threads * norm_backward_rows(s), 0, st>>>(b);
+            });
+        });
     });
 }
 
