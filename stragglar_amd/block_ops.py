@@ -33,6 +33,11 @@ class Routing:
     __slots__ = ("row_of_slot", "slot_of_row", "offsets", "num_experts", "ranks")
 
     def __init__(self, row_of_slot, slot_of_row, offsets, num_experts: int, ranks: int):
+        if row_of_slot.dim() != 2 or slot_of_row.numel() != row_of_slot.numel() or offsets.numel() != num_experts + 1 or num_experts % ranks:
+            raise ValueError("row_of_slot [tokens, topk], slot_of_row [tokens * topk] and offsets [num_experts + 1] do not fit each other")
+        for t in (row_of_slot, slot_of_row, offsets):
+            if t.dtype is not torch.int32 or not t.is_contiguous() or t.device != offsets.device:
+                raise ValueError("a routing is made of contiguous int32 tensors on one device")
         self.row_of_slot, self.slot_of_row, self.offsets = row_of_slot, slot_of_row, offsets
         self.num_experts, self.ranks = num_experts, ranks
 

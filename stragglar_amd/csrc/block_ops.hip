@@ -390,7 +390,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(const I* __r
         const bool in = key[s] != kDropped;
         const uint32_t row = in ? first[key[s]] + seen[wave * num_experts + key[s]] + place[s] : kDropped;
         row_of_slot[slot] = (int32_t)row;
-        if (in) slot_of_row[row] = (int32_t)slot;
+        if (row < n) slot_of_row[row] = (int32_t)slot;            // (expert numbers that change between the launches)
         if (slot >= total) slot_of_row[slot] = -1;               // the rows behind the last one
     }
 }

@@ -33,6 +33,16 @@ def test_route_refuses(group):
             group.route(bad, experts)
 
 
+def test_routing_refuses():
+    i = lambda *shape: torch.zeros(*shape, dtype=torch.int32)
+    for args in [(i(6), i(6), i(9), 8, 4), (i(3, 2), i(5), i(9), 8, 4), (i(3, 2), i(6), i(8), 8, 4), (i(3, 2), i(6), i(9), 8, 3),
+                 (i(3, 2).long(), i(6), i(9), 8, 4), (i(2, 3).t(), i(6), i(9), 8, 4), (i(3, 2), i(6), i(9).float(), 8, 4)]:
+        with pytest.raises(ValueError):
+            block_ops.Routing(*args)
+    r = block_ops.Routing(i(3, 2), i(6), torch.arange(9, dtype=torch.int32), 8, 4)
+    assert (r.tokens, r.topk) == (3, 2) and r.rank_offsets.tolist() == [0, 2, 4, 6, 8]
+
+
 def test_dispatch_and_combine_refuse(group):
     r = routing()
     for call, why in [(lambda: group.dispatch(torch.zeros(4, 8), r), "tokens must be"),

@@ -446,6 +446,70 @@ def test_reduce_norm_of_zeros_infinities_and_nan(groups):
     assert torch.allclose(normed.float(), torch.ones_like(normed.float()), rtol=0, atol=2 ** -10)
 
 
+def test_more_rows_than_one_pass_of_the_grid(groups):
+    """Row counts at which every kernel's grid goes round: 2^20 workgroups of norms, 2^20 of four tokens."""
+    g = groups(4)
+    x, res, w = randn(1, 1100003, 8, dtype=torch.float16), randn(2, 1100003, 8, dtype=torch.float16), randn(3, 8, mean=1.0, scale=0.1)
+    gh, gx = randn(4, 1100003, 8, dtype=torch.float16), randn(5, 1100003, 8, dtype=torch.float16)
+    s = dict(partials=x, residual=res, pre_weight=w, post_weight=w, gate=w)
+    with torch.no_grad():
+        hidden, normed, saved = run_norm(g, s, 0.5, 1e-6, False, save=True)
+        back = g.reduce_norm_backward(saved, gh, gx)
+    h, n, want = plain_norm(s, 0.5, 1e-6, gh, gx.unsqueeze(0))
+    check(hidden, h, "hidden"), check(normed, n, "normed"), check(back.partials, want["partials"], "partials")
+    # column sums: 1100003 tokens over 512 workgroups of 8 rows is 269 additions in a row, in front of the rest of COLUMN
+    for k in ("pre_weight", "post_weight", "gate"):
+        check(getattr(back, k), B(want[k].v, want[k].e * 4), k)
+    t = 4200003
+    e = choices(6, t, 1, 8, 0.1)
+    r = g.route(e, 8)
+    assert_route(r, e, 8)
+    rows, wt, gy = randn(7, t, 8, dtype=torch.bfloat16), randn(8, t, 1), randn(9, t, 8, dtype=torch.bfloat16)
+    index, has = r.row_of_slot.long()[:, 0], r.row_of_slot[:, 0] >= 0
+    y = g.combine(rows, r, wt)
+    taken = torch.where(has.unsqueeze(1), rows.double()[index.clamp(min=0)], torch.zeros((), dtype=torch.float64, device="cuda"))
+    check(y, B(taken) * B(wt), "combine")
+    gr, gw = g.combine_backward(gy, rows, r, wt)
+    check(gw, (B(gy) * B(taken)).sum(1, 16, keepdim=True), "grad_weights")
+    check(gr[index[has]], B(gy[has]) * B(wt[has]), "grad_rows")
+    assert not gr[int(r.offsets[-1]):].any()
+    assert torch.equal(g.dispatch(gy, r)[index[has]], gy[has])
+
+
+def test_row_numbers_out_of_range_count_as_dropped(groups):
+    """A routing whose numbers were overwritten: the kernels hold every row number against the number of rows."""
+    from stragglar_amd.block_ops import Routing
+    g = groups(4)
+    r = g.route(choices(1, 10, 2, 8), 8)
+    rows = r.row_of_slot.clone()
+    rows[3, 0], rows[5, 1], rows[7, 0] = 20, -12345, 2 ** 31 - 1
+    offsets = r.offsets.clone()
+    offsets[-1] = 2 ** 31 - 1
+    bad = Routing(rows, r.slot_of_row, offsets, 8, 4)
+    x, w = randn(2, 10, 24), torch.ones(10, 2, device="cuda")
+    out = g.dispatch(x, bad)
+    keep = torch.ones(10, 2, dtype=torch.bool, device="cuda")
+    keep[3, 0] = keep[5, 1] = keep[7, 0] = False
+    src = randn(3, 20, 24)
+    want = (src[r.row_of_slot.long()] * keep.unsqueeze(2)).sum(1)
+    assert torch.equal(out[r.row_of_slot[keep].long()], x.unsqueeze(1).expand(-1, 2, -1)[keep])
+    assert torch.equal(g.combine(src, bad, w), want)
+    gr, gw = g.combine_backward(x, src, bad, w)
+    assert not gw[~keep].any() and torch.equal(gr[r.row_of_slot[keep].long()], x.unsqueeze(1).expand(-1, 2, -1)[keep])
+
+
+def test_not_differentiable_twice(groups):
+    g = groups(4)
+    x = randn(1, 6, 16).requires_grad_(True)
+    r = g.route(choices(2, 6, 2, 8), 8)
+    w = torch.softmax(randn(3, 6, 2), 1).requires_grad_(True)
+    hidden, normed = g.reduce_norm(x, x.detach(), pre_weight=torch.ones(16, device="cuda"), gather=False)
+    for out, leaf in [(g.dispatch(x, r), x), (g.combine(g.dispatch(x, r).detach(), r, w), w), (normed, x)]:
+        grad, = torch.autograd.grad(out.square().sum(), leaf, create_graph=True)      # once is fine
+        with pytest.raises(RuntimeError, match="once_differentiable|twice"):
+            grad.sum().backward()
+
+
 # ---- together, and in a program ----------------------------------------------------------------------------------
 
 def block(g, partials, residual, experts, weights, mats, w, gate, num_experts):
