@@ -205,13 +205,13 @@ def _combine_backward(group, grad, rows, routing, weights, want_rows, want_weigh
 
 class _Dispatch(_Node):
     @staticmethod
-    def forward(ctx, rows, group, routing):
-        ctx.group, ctx.routing = group, routing
-        return _dispatch(group, rows, routing)
+    def forward(ctx, rows, plain):
+        ctx.plain = plain
+        return _dispatch(plain[0], rows, plain[1])
 
     @staticmethod
     def gradients(ctx, grad):
-        return _combine(ctx.group, grad.contiguous(), ctx.routing), None, None
+        return _combine(ctx.plain[0], grad.contiguous(), ctx.plain[1]), None
 
     @staticmethod
     def backward(ctx, grad):
@@ -220,17 +220,17 @@ class _Dispatch(_Node):
 
 class _Combine(_Node):
     @staticmethod
-    def forward(ctx, rows, weights, group, routing):
-        ctx.group, ctx.routing = group, routing
+    def forward(ctx, rows, weights, plain):
+        ctx.plain = plain
         ctx.save_for_backward(rows, weights)
-        return _combine(group, rows, routing, weights)
+        return _combine(plain[0], rows, plain[1], weights)
 
     @staticmethod
     def gradients(ctx, grad):
         rows, weights = ctx.saved_tensors
         need = ctx.needs_input_grad
-        a, b = _combine_backward(ctx.group, grad.contiguous(), rows, ctx.routing, weights, need[0], weights is not None and need[1])
-        return a, b, None, None
+        a, b = _combine_backward(ctx.plain[0], grad.contiguous(), rows, ctx.plain[1], weights, need[0], weights is not None and need[1])
+        return a, b, None
 
     @staticmethod
     def backward(ctx, grad):
@@ -259,7 +259,7 @@ def dispatch(group, tokens, routing):
     _routing_rows(group, "tokens", tokens, routing, False)
     _on_device(group, tokens=tokens, routing=routing.offsets)
     if _recording(tokens):
-        return _Dispatch.apply(tokens, group, routing)
+        return _Dispatch.apply(tokens, (group, routing))
     return _dispatch(group, tokens, routing)
 
 
@@ -268,7 +268,7 @@ def combine(group, rows, routing, weights=None):
     _check_weights(routing, weights, rows.dtype)
     _on_device(group, rows=rows, weights=weights, routing=routing.offsets)
     if _recording(rows, weights):
-        return _Combine.apply(rows, weights, group, routing)
+        return _Combine.apply(rows, weights, (group, routing))
     return _combine(group, rows, routing, weights)
 
 
@@ -350,21 +350,21 @@ def _reduce_norm_backward(group, s: ReduceNormSaved, grad_hidden, grad_normed, w
         torch.empty_like(gate) if want[4] and gate is not None else None)
     lib = group._lib
     need = _norm_workspace(tokens, dim, args.dtype)
-    work = torch.empty(need // 4, dtype=torch.float32, device=residual.device)
+    work = torch.empty(need // 4, dtype=torch.float32, device=residual.device) if need else None
     # total, total_dtype, reserved, then the gradients that come in, those that go out, and the workspace
     grads = capi.ReduceNormGrads(total.data_ptr(), DTYPE_CODES[total.dtype], 0, _ptr(grad_hidden), _ptr(grad_normed), _ptr(out[0]), _ptr(out[1]),
-                                 _ptr(out[2]), _ptr(out[3]), _ptr(out[4]), work.data_ptr(), need)
+                                 _ptr(out[2]), _ptr(out[3]), _ptr(out[4]), _ptr(work), need)
     lib.check(lib.lib.sar_reduce_norm_backward(group.device, _raw_stream(group.device), ctypes.byref(args), ctypes.byref(grads)))
     return out
 
 
 class _ReduceNorm(_Node):
     @staticmethod
-    def forward(ctx, group, shape, residual_scale, eps, gather, residual, pre_weight, post_weight, gate, *partials):
+    def forward(ctx, plain, residual, pre_weight, post_weight, gate, *partials):
+        group, shape, residual_scale, eps, gather = plain
         rows = partials[0] if len(shape) == 3 and len(partials) == 1 else partials
         hidden, normed, total, stats = _reduce_norm(group, rows, residual, pre_weight, post_weight, gate, residual_scale, eps, gather, True)
-        ctx.group, ctx.inputs = group, len(partials)
-        ctx.plain = (group.n if len(shape) == 3 else 1, group.n if gather else 1, shape, residual_scale, eps)
+        ctx.plain = plain
         ctx.save_for_backward(total, stats, residual, pre_weight, post_weight, gate)
         ctx.set_materialize_grads(False)
         return hidden, normed
@@ -372,49 +372,40 @@ class _ReduceNorm(_Node):
     @staticmethod
     def gradients(ctx, grad_hidden, grad_normed):
         total, stats, residual, pre_weight, post_weight, gate = ctx.saved_tensors
-        sources, copies, shape, scale, eps = ctx.plain
-        saved = ReduceNormSaved(sources, copies, shape, total, stats, residual, pre_weight, post_weight, gate, scale, eps)
+        group, shape, residual_scale, eps, gather = ctx.plain
+        saved = ReduceNormSaved(group.n if len(shape) == 3 else 1, group.n if gather else 1, shape, total, stats, residual, pre_weight,
+                                post_weight, gate, residual_scale, eps)
         need = ctx.needs_input_grad
-        g = _reduce_norm_backward(ctx.group, saved, grad_hidden.contiguous() if grad_hidden is not None else None,
-                                  grad_normed.contiguous() if grad_normed is not None else None, (True in need[9:], need[5], need[6], need[7], need[8]))
-        if g[0] is None:
-            partials = (None,) * ctx.inputs
-        elif ctx.inputs == 1:
-            partials = (g[0],)
-        else:
-            partials = g[0].unbind(0)
-        return (None, None, None, None, None, g[1], g[2], g[3], g[4], *partials)
+        g = _reduce_norm_backward(group, saved, grad_hidden.contiguous() if grad_hidden is not None else None,
+                                  grad_normed.contiguous() if grad_normed is not None else None, (True in need[5:], need[1], need[2], need[3], need[4]))
+        inputs = len(need) - 5
+        if inputs == 1:
+            return None, g[1], g[2], g[3], g[4], g[0]
+        return (None, g[1], g[2], g[3], g[4], *(g[0].unbind(0) if g[0] is not None else (None,) * inputs))
 
     @staticmethod
     def backward(ctx, grad_hidden, grad_normed):
         return _ReduceNorm._backward(ctx, grad_hidden, grad_normed)
 
 
-def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], residual, pre_weight=None, post_weight=None, gate=None,
-                residual_scale: float = 1.0, eps: float = 1e-6, gather: bool = True, save: bool = False):
+def _check_reduce_norm(group, partials, inputs, residual, pre_weight, post_weight, gate, eps):
+    """Says what is wrong with the arguments of reduce_norm."""
     if not isinstance(residual, torch.Tensor) or residual.dim() != 2:
         raise ValueError("residual must be a tensor [tokens, dim]")
     _tensor("residual", residual, dtypes=DTYPE_CODES)
-    size = residual.shape
-    tokens, dim = size
-    dtype, device = residual.dtype, group.device
+    (tokens, dim), dtype = residual.shape, residual.dtype
     if not 1 <= dim <= MAX_NORM_DIM:
         raise ValueError("dim must be 1 to %d, got %d" % (MAX_NORM_DIM, dim))
     if isinstance(partials, torch.Tensor):
-        inputs = (partials,)
-        if partials.dim() not in (2, 3) or partials.shape[-2:] != size or (partials.dim() == 3 and partials.shape[0] != group.n):
+        if partials.dim() not in (2, 3) or partials.shape[-2:] != residual.shape or (partials.dim() == 3 and partials.shape[0] != group.n):
             raise ValueError("partials must be [%d ranks, tokens, dim] or, as a finished output, [tokens, dim]: got %s with residual %s"
-                             % (group.n, tuple(partials.shape), tuple(size)))
+                             % (group.n, tuple(partials.shape), tuple(residual.shape)))
         _tensor("partials", partials, dtypes=(dtype,))
-        shape = tuple(partials.shape)
     else:
-        inputs = tuple(partials)
         if len(inputs) != group.n:
             raise ValueError("need one partial output per emulated rank: %d, got %d" % (group.n, len(inputs)))
         for p in inputs:
-            if not isinstance(p, torch.Tensor) or p.dtype is not dtype or p.shape != size or not p.is_contiguous():
-                _tensor("a partial output", p, size, (dtype,))
-        shape = (group.n, tokens, dim)
+            _tensor("a partial output", p, residual.shape, (dtype,))
     kinds = (torch.float32, dtype)
     if pre_weight is not None:
         _tensor("pre_weight", pre_weight, (dim,), kinds)
@@ -426,13 +417,48 @@ def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], re
             raise ValueError("gate must be [dim], [tokens, 1] or [tokens, dim]: got %s" % (tuple(gate.shape),))
     if not 0 <= eps < float("inf"):
         raise ValueError("eps must be a finite number, zero or more")
-    for t in (residual, pre_weight, post_weight, gate) + inputs:
-        if t is not None and t.get_device() != device:
-            raise ValueError("every tensor must be a CUDA tensor on device %d" % device)
+    for t in (residual, pre_weight, post_weight, gate, *inputs):
+        if t is not None and t.get_device() != group.device:
+            raise ValueError("every tensor must be a CUDA tensor on device %d" % group.device)
+
+
+def _fits_reduce_norm(group, partials, inputs, residual, pre_weight, post_weight, gate, eps):
+    """The checks above in as little time as they take."""
+    if not isinstance(residual, torch.Tensor) or residual.dim() != 2:
+        return False
+    size, dtype, device = residual.shape, residual.dtype, group.device
+    dim = size[1]
+    if dtype not in DTYPE_CODES or not 1 <= dim <= MAX_NORM_DIM or not residual.is_contiguous() or residual.get_device() != device or not 0 <= eps < float("inf"):
+        return False
+    if isinstance(partials, torch.Tensor):
+        if partials.shape != size and partials.shape != (group.n, *size):
+            return False
+        size = partials.shape
+    elif len(inputs) != group.n:
+        return False
+    for p in inputs:
+        if not isinstance(p, torch.Tensor) or p.dtype is not dtype or p.shape != size or not p.is_contiguous() or p.get_device() != device:
+            return False
+    for w in (pre_weight, post_weight):
+        if w is not None and (not isinstance(w, torch.Tensor) or w.dim() != 1 or w.shape[0] != dim or not w.is_contiguous() or w.get_device() != device
+                              or (w.dtype is not dtype and w.dtype is not torch.float32)):
+            return False
+    return gate is None or (isinstance(gate, torch.Tensor) and gate.is_contiguous() and gate.get_device() == device
+                            and (gate.dtype is dtype or gate.dtype is torch.float32)
+                            and tuple(gate.shape) in ((dim,), (residual.shape[0], 1), (residual.shape[0], dim)))
+
+
+def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], residual, pre_weight=None, post_weight=None, gate=None,
+                residual_scale: float = 1.0, eps: float = 1e-6, gather: bool = True, save: bool = False):
+    inputs = (partials,) if isinstance(partials, torch.Tensor) else tuple(partials)
+    if not _fits_reduce_norm(group, partials, inputs, residual, pre_weight, post_weight, gate, eps):
+        _check_reduce_norm(group, partials, inputs, residual, pre_weight, post_weight, gate, eps)
+        raise ValueError("the arguments do not fit each other")
+    shape = tuple(partials.shape) if inputs[0] is partials else (group.n, *residual.shape)
     if _recording(residual, pre_weight, post_weight, gate, *inputs):
         if save:
             raise ValueError("save=True is for calls under torch.no_grad(): autograd keeps what it needs by itself")
-        return _ReduceNorm.apply(group, shape, residual_scale, eps, gather, residual, pre_weight, post_weight, gate, *inputs)
+        return _ReduceNorm.apply((group, shape, residual_scale, eps, gather), residual, pre_weight, post_weight, gate, *inputs)
     rows = partials if len(shape) == 3 and len(inputs) == 1 else inputs
     hidden, normed, total, stats = _reduce_norm(group, rows, residual, pre_weight, post_weight, gate, residual_scale, eps, gather, save)
     if not save:

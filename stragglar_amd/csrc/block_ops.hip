@@ -752,7 +752,7 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_kernel(const NormArg
 //   d partials = r1 (du post - yhat mean(du post yhat))
 // hidden is computed again from y and the residual, so nothing that was rounded comes back.  A workgroup walks over
 // tokens and keeps the column sums in registers; they leave as one row of sums per workgroup, added up by
-// column_sum_kernel in a fixed order.
+// column_sum_kernel in a fixed order; a single workgroup writes the gradients itself.
 struct NormBackwardArgs {
     NormArgs f;
     const char* total;
@@ -761,8 +761,9 @@ struct NormBackwardArgs {
     char* grad_partials;
     char* grad_residual;
     char* grad_gate;                   // per token or full (a channel gate's gradient is a column sum)
-    float* columns;                    // [workgroup][3][dim]
-    uint32_t total_f32, want_pre, want_post, want_gate;   // want_gate: a channel gate's
+    float* columns;                    // [workgroup][3][dim], unless there is only one
+    char* grad_weights[3];             // of pre, post and a channel gate: null = not wanted
+    uint32_t weights_f32[3], total_f32;
     uint32_t row_threads;              // threads of one row
 };
 
@@ -950,11 +951,12 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
                     for (int i = 0; i < VE; ++i) x[0][i] += rows[(m * r.step + r.at) * VE + i];
             }
         }
-        store_params<DT, VE, V>((char*)(b.columns + ((uint64_t)blockIdx.x * 3u + which) * a.dim), true, x, a, r);
+        if (gridDim.x == 1) store_params<DT, VE, V>(b.grad_weights[which], b.weights_f32[which], x, a, r);
+        else store_params<DT, VE, V>((char*)(b.columns + ((uint64_t)blockIdx.x * 3u + which) * a.dim), true, x, a, r);
     };
-    if (b.want_pre) leave(col_pre, 0);
-    if (b.want_post) leave(col_post, 1);
-    if (b.want_gate) leave(col_gate, 2);
+    if (b.grad_weights[0]) leave(col_pre, 0);
+    if (b.grad_weights[1]) leave(col_post, 1);
+    if (b.grad_weights[2]) leave(col_gate, 2);
 }
 
 // Adds the workgroups' rows of column sums: 32 columns a workgroup, 32 groups of threads taking every 32nd row, then in
@@ -1383,7 +1385,8 @@ int sar_reduce_norm(int device, void* stream, const sar_reduce_norm_args* args) 
 
 uint64_t sar_reduce_norm_workspace(int64_t tokens, int64_t dim, int dtype) {
     if (tokens < 0 || dim < 1 || dim > SAR_MAX_NORM_DIM || !known_dtype(dtype)) return 0;
-    return (uint64_t)norm_backward_groups(tokens, dim, dtype) * 3u * (uint64_t)dim * 4u;
+    const uint64_t groups = norm_backward_groups(tokens, dim, dtype);
+    return groups == 1 ? 0 : groups * 3u * (uint64_t)dim * 4u;
 }
 
 int sar_reduce_norm_backward(int device, void* stream, const sar_reduce_norm_args* forward, const sar_reduce_norm_grads* g) {
@@ -1404,7 +1407,8 @@ int sar_reduce_norm_backward(int device, void* stream, const sar_reduce_norm_arg
             !aligned(g->grad_post_weight, g->grad_post_weight ? elem_size(forward->post_dtype) : 1) ||
             !aligned(g->grad_gate, g->grad_gate ? elem_size(forward->gate_dtype) : 1))
             return refuse("a pointer is not aligned to its element size");
-        if (!g->workspace || !aligned(g->workspace, 4) || g->workspace_bytes < sar_reduce_norm_workspace(forward->tokens, forward->dim, forward->dtype))
+        const uint64_t need = sar_reduce_norm_workspace(forward->tokens, forward->dim, forward->dtype);
+        if (need && (!g->workspace || !aligned(g->workspace, 4) || g->workspace_bytes < need))
             return refuse("the workspace is smaller than sar_reduce_norm_workspace()");
         OnDevice on(device);
         if (on.error() != hipSuccess) return not_current(device, on.error());
@@ -1418,23 +1422,21 @@ int sar_reduce_norm_backward(int device, void* stream, const sar_reduce_norm_arg
         b.grad_residual = (char*)g->grad_residual;
         b.grad_gate = channel ? nullptr : (char*)g->grad_gate;
         b.columns = (float*)g->workspace;
-        b.want_pre = g->grad_pre_weight != nullptr;
-        b.want_post = g->grad_post_weight != nullptr;
-        b.want_gate = channel && g->grad_gate != nullptr;
+        b.grad_weights[0] = (char*)g->grad_pre_weight;
+        b.grad_weights[1] = (char*)g->grad_post_weight;
+        b.grad_weights[2] = channel ? (char*)g->grad_gate : nullptr;
+        b.weights_f32[0] = b.f.pre_f32;
+        b.weights_f32[1] = b.f.post_f32;
+        b.weights_f32[2] = b.f.gate_f32;
         const uint32_t groups = norm_backward_groups(forward->tokens, forward->dim, forward->dtype);
         const NormShape shape = norm_shape(forward->dtype, forward->dim);
         b.row_threads = shape.threads;
         with_dtype(forward->dtype, [&](auto dt) { launch_norm_backward<decltype(dt)::value>((hipStream_t)stream, b, shape, groups); });
         if (int rc = launched("sar_reduce_norm_backward")) return rc;
-        if (b.want_pre || b.want_post || b.want_gate) {
+        if (groups > 1 && (b.grad_weights[0] || b.grad_weights[1] || b.grad_weights[2])) {
             ColumnArgs c{};
             c.columns = b.columns;
-            c.out[0] = (char*)g->grad_pre_weight;
-            c.out[1] = (char*)g->grad_post_weight;
-            c.out[2] = channel ? (char*)g->grad_gate : nullptr;
-            c.f32[0] = b.f.pre_f32;
-            c.f32[1] = b.f.post_f32;
-            c.f32[2] = b.f.gate_f32;
+            for (int i = 0; i < 3; ++i) { c.out[i] = b.grad_weights[i]; c.f32[i] = b.weights_f32[i]; }
             c.rows = groups;
             c.dim = b.f.dim;
             const dim3 grid((c.dim + 31u) / 32u, 3);

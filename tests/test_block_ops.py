@@ -170,9 +170,9 @@ def test_c_entries_refuse(sarlib):
     for g, why in [(dict(grad_normed=p), "without pre_weight"), (dict(grad_pre_weight=p), "without pre_weight"), (dict(grad_post_weight=p), "without post_weight"),
                    (dict(grad_gate=p), "without a gate"), (dict(total=None), "null"), (dict(total_dtype=2), "total"), (dict(workspace=None), "workspace"),
                    (dict(workspace_bytes=16), "workspace"), (dict(grad_hidden=odd), "aligned")]:
-        refused(sarlib, norm(backward=True, grads=g), why)
+        refused(sarlib, norm(backward=True, grads=g, tokens=100), why)
     refused(sarlib, norm(backward=True, stats=None), "null")
-    assert L.sar_reduce_norm_workspace(4, 8, 0) >= 3 * 8 * 4 and L.sar_reduce_norm_workspace(4, 0, 0) == 0
+    assert L.sar_reduce_norm_workspace(100, 8, 0) >= 3 * 8 * 4 and L.sar_reduce_norm_workspace(1, 8, 0) == 0 and L.sar_reduce_norm_workspace(4, 0, 0) == 0
 
 
 def test_struct_sizes_follow_the_header(tmp_path):

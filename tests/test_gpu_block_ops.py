@@ -476,6 +476,62 @@ def test_more_rows_than_one_pass_of_the_grid(groups):
     assert torch.equal(g.dispatch(gy, r)[index[has]], gy[has])
 
 
+@pytest.mark.parametrize("dtype,dim", [("bf16", 4096), ("f16", 2050), ("f32", 1028)])
+def test_calls_large_enough_to_stream(groups, dtype, dim):
+    """Calls of 512 MiB and more go past the caches, in kernels of their own: every kind of call at such a size, looked at in
+    a few places."""
+    n, dt = 8, DT[dtype]
+    g = groups(n)
+    es = torch.finfo(dt).bits // 8
+    t = (600 << 20) // (18 * dim * es)
+    base = [randn(r, 499, dim, dtype=dt) for r in range(4)]
+    spread = torch.arange(t, device="cuda")
+    s = dict(partials=[base[r % 4][(spread * (r + 1) + r) % 499] for r in range(n)], residual=base[3][(spread * 3) % 499],
+             pre_weight=randn(5, dim, mean=1.0, scale=0.2), post_weight=randn(6, dim, mean=1.0, scale=0.2), gate=randn(7, dim, mean=0.5, scale=0.2))
+    gh, gx = base[0][(spread * 7) % 499], torch.stack([base[r % 4][(spread * 11 + r) % 499] for r in range(n)])
+    with torch.no_grad():
+        hidden, normed, saved = run_norm(g, s, 0.75, 1e-6, True, save=True)
+        back = g.reduce_norm_backward(saved, gh, gx)
+    for a in (0, t // 2, t - 30):
+        part = slice(a, a + 30)
+        h, x, want = plain_norm(dict(s, partials=[p[part] for p in s["partials"]], residual=s["residual"][part]), 0.75, 1e-6, gh[part], gx[:, part])
+        check(hidden[part], h, a), check(back.residual[part], want["residual"], a)
+        for r in range(n):
+            check(normed[r, part], x, (a, r)), check(back.partials[r, part], want["partials"], (a, r))
+    # the column sums, over all tokens
+    sums = {k: torch.zeros(dim, dtype=torch.float64, device="cuda") for k in ("pre_weight", "post_weight", "gate")}
+    bounds = {k: torch.zeros(dim, dtype=torch.float64, device="cuda") for k in sums}
+    for a in range(0, t, 1000):
+        part = slice(a, min(t, a + 1000))
+        want = plain_norm(dict(s, partials=[p[part] for p in s["partials"]], residual=s["residual"][part]), 0.75, 1e-6, gh[part], gx[:, part])[2]
+        for k in sums:
+            sums[k] += want[k].v
+            bounds[k] += want[k].e
+    for k in sums:
+        check(getattr(back, k), B(sums[k], bounds[k]), k)
+    del hidden, normed, saved, back, gx, s
+    topk = 4
+    t = (560 << 20) // (topk * dim * es)
+    r = g.route(choices(1, t, topk, 16, 0.05), 16)
+    x = base[0][torch.arange(t, device="cuda") % 499]
+    rows = g.dispatch(x, r)
+    slots = r.slot_of_row.long()
+    want = torch.where((slots >= 0).unsqueeze(1), x[slots.clamp(min=0) // topk], torch.zeros((), dtype=dt, device="cuda"))
+    assert torch.equal(rows, want)
+    del want
+    w = torch.softmax(randn(3, t, topk), 1)
+    y = g.combine(rows, r, w)
+    gr, gw = g.combine_backward(x, rows, r, w)
+    assert not gr[int(r.offsets[-1]):].any()
+    for a in (0, t // 2, t - 30):
+        part = slice(a, a + 30)
+        index, has = r.row_of_slot[part].long(), r.row_of_slot[part] >= 0
+        taken = torch.where(has.unsqueeze(2), rows[index.clamp(min=0)].double(), torch.zeros((), dtype=torch.float64, device="cuda"))
+        check(y[part], (B(taken) * B(w[part].unsqueeze(2))).sum(1, topk), a)
+        check(gw[part], (B(x[part].unsqueeze(1).expand_as(taken)) * B(taken)).sum(2, dim // 64 + 64), a)
+        check(gr[index[has]], B(x[part].unsqueeze(1).expand(-1, topk, -1)[has]) * B(w[part][has].unsqueeze(1)), a)
+
+
 def test_row_numbers_out_of_range_count_as_dropped(groups):
     """A routing whose numbers were overwritten: the kernels hold every row number against the number of rows."""
     from stragglar_amd.block_ops import Routing
