@@ -444,7 +444,7 @@ __global__ __launch_bounds__(kMoveThreads) void dispatch_kernel(const MoveArgs a
         const char* const from = a.in + token * a.row_bytes;
         R v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = load<DT, VE, NT>(from, Place<DT, VE>(v0 + u * kWave, a.nvec, a.dim).byte());
+        for (int u = 0; u < U; ++u) v[u] = load<DT, VE>(from, Place<DT, VE>(v0 + u * kWave, a.nvec, a.dim).byte());
         for (uint64_t left = __ballot(lane < a.topk && listed < a.nrows); left; left &= left - 1) {
             const int k = __builtin_ctzll(left);
             char* const to = a.out + (uint64_t)lane_value(listed, k) * a.row_bytes;
@@ -698,7 +698,7 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_kernel(const NormArg
     float post[V][VE], pre[V][VE], gate[V][VE];
     for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
         const uint64_t at = token * a.row_bytes;
-        const auto res = load_row<DT, VE, V, NT>(a.residual + at, a, r);
+        const auto res = load_row<DT, VE, V>(a.residual + at, a, r);
         if (kEarly) {
             if (a.post) load_params<DT, VE, V>(a.post, a.post_f32, a, r, post);
             if (a.gate_kind == SAR_GATE_CHANNEL) load_params<DT, VE, V>(a.gate, a.gate_f32, a, r, gate);
@@ -729,7 +729,7 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_kernel(const NormArg
 #pragma unroll
             for (int i = 0; i < VE; ++i) x[v][i] = fmaf(a.residual_scale, h[i], a.gate_kind == SAR_GATE_NONE ? x[v][i] : gate[v][i] * x[v][i]);
         }
-        if (a.hidden) store_row<DT, VE, V, NT>(a.hidden + at, 0, 1, x, a, r);
+        if (a.hidden) store_row<DT, VE, V, false>(a.hidden + at, 0, 1, x, a, r);
         float r2 = 1.f;
         if (a.pre) {
             r2 = dot_row<DT, VE, V>(x, x, a, r);
@@ -1093,7 +1093,9 @@ MoveArgs move_args(int dtype, int64_t tokens, int topk, int64_t dim, const int32
 // Cache only pushes out what does, and a cached store's way to memory is paid for by the next call.  Measured, cached
 // against streaming, as a chain with a pass over the result behind it: dispatch of 537 MB 407 against 381 us (chain
 // with its combine), of 268 MB 173 against 184; eight partials of 8192 x 4096 (1.2 GB) 432 against 397, of 4096 222
-// against 213, of 2048 (302 MB) 107 against 118.
+// against 213, of 2048 (302 MB) 107 against 118.  The streams that come once beside eight others stay cached all the same:
+// dispatch's tokens (230 -> 212 us with its gradient), the residual and hidden of reduce_norm (221 -> 205), its total for the
+// backward pass (287 -> 272).
 constexpr uint64_t kStreamBytes = 512ull << 20;
 
 // calls f(integral_constant<bool, B>)
