@@ -236,6 +236,10 @@ __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__bui
 // Few slots: one workgroup does it all in one launch.  More: one launch counts the slots of each expert in every block
 // of kRouteBlock slots and one places them, every block adding up the counts of the blocks before it.  Many blocks:
 // that sum, which grows with the square of the blocks, becomes a launch of its own.
+// Bound by latency, not by bytes: 128 slots 2.7 us (a launch), 8192 over 256 experts 11.5 (two launches would take 9.3 on the
+// GPU and 2 more on the host), 131072 12.6 (with the sum in a launch of its own 12.9, and 8 more on the host), 1048576 over
+// 256 19.8 (adding up in every block: 32), of which 17 MB at the card's copy rate are 3.  Blocks of 2048 slots were faster up
+// to 131072 (9 us) and slower above (27 at 524288), blocks of 8192 slower everywhere below a million.
 constexpr uint32_t kRouteThreads = 1024, kRouteWaves = kRouteThreads / kWave;
 constexpr uint32_t kRouteOneStrips = 8, kRouteStrips = 4;
 constexpr uint32_t kRouteOne = kRouteThreads * kRouteOneStrips, kRouteBlock = kRouteThreads * kRouteStrips;
@@ -396,9 +400,12 @@ __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(const I* __r
 }
 
 // ---- dispatch, combine --------------------------------------------------------------------------------------
-// A wave takes one token (and a segment of 64 * U vectors of its row).  Lane k holds the row and the weight of choice k;
+// A wave takes one token (and 64 vectors of its row).  Lane k holds the row and the weight of choice k;
 // the choices that were not dropped are the bits of a ballot, walked in order with the row number in a scalar register.
 // Row numbers come from memory and are held against the number of rows before they become an address.
+// Bound by HBM: 16384 tokens of 2048 in bf16, eight choices (0.6 GB): dispatch 105 us, 5.7 TB/s (a torch copy of that size
+// 5.1), combine 101 us, 6.0 TB/s.  Consecutive tokens per XCD instead of round robin changed nothing (231 against 236 us for
+// both).
 constexpr uint32_t kMoveThreads = 256, kMoveWaves = kMoveThreads / kWave;
 
 struct MoveArgs {
@@ -431,88 +438,68 @@ __device__ __forceinline__ void zero_rows(const MoveArgs& a, uint64_t token, uin
 __device__ __forceinline__ uint32_t lane_value(uint32_t x, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, lane); }
 __device__ __forceinline__ float lane_value(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
 
-template <int DT, int VE, int U, bool NT, bool WEIGHTED>
+template <int DT, int VE, bool NT, bool WEIGHTED>
 __global__ __launch_bounds__(kMoveThreads) void dispatch_kernel(const MoveArgs a) {
     typedef typename Raw<DT, VE>::T R;
-    const uint32_t lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
-    const uint32_t v0 = blockIdx.x * (U * kWave) + lane;
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave), vec = blockIdx.x * kWave + lane;
+    const Place<DT, VE> p(vec, a.nvec, a.dim);
     for (uint64_t token = (uint64_t)blockIdx.y * kMoveWaves + wave; token < a.tokens; token += (uint64_t)gridDim.y * kMoveWaves) {
         const uint64_t slot = token * a.topk + min(lane, a.topk - 1);
         const uint32_t listed = (uint32_t)a.row_of_slot[slot];
         float weight = 1.f;
         if (WEIGHTED) weight = load_one<DT>(a.weights, a.weights_f32, slot);
-        const char* const from = a.in + token * a.row_bytes;
-        R v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = load<DT, VE>(from, Place<DT, VE>(v0 + u * kWave, a.nvec, a.dim).byte());
+        const R v = load<DT, VE>(a.in + token * a.row_bytes, p.byte());
         for (uint64_t left = __ballot(lane < a.topk && listed < a.nrows); left; left &= left - 1) {
             const int k = __builtin_ctzll(left);
             char* const to = a.out + (uint64_t)lane_value(listed, k) * a.row_bytes;
-            const float w = WEIGHTED ? lane_value(weight, k) : 1.f;
+            R r = v;
+            if constexpr (WEIGHTED) {
+                const float w = lane_value(weight, k);
+                float x[VE];
+                unpack<DT, VE>(r, x);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const Place<DT, VE> p(v0 + u * kWave, a.nvec, a.dim);
-                R r = v[u];
-                if constexpr (WEIGHTED) {
-                    float x[VE];
-                    unpack<DT, VE>(r, x);
-#pragma unroll
-                    for (int i = 0; i < VE; ++i) x[i] *= w;
-                    r = pack<DT, VE>(x);
-                }
-                if (p.in) store<DT, VE, NT>(to, p.byte(), r);
+                for (int i = 0; i < VE; ++i) x[i] *= w;
+                r = pack<DT, VE>(x);
             }
+            if (p.in) store<DT, VE, NT>(to, p.byte(), r);
         }
-        zero_rows<DT, VE, U, NT>(a, token, v0);
+        zero_rows<DT, VE, 1, NT>(a, token, vec);
     }
 }
 
 // The sum is kept in 32 bits and taken in the order of the choices.
-template <int DT, int VE, int U, bool NT>
+template <int DT, int VE, bool NT>
 __global__ __launch_bounds__(kMoveThreads) void combine_kernel(const MoveArgs a) {
-    typedef typename Raw<DT, VE>::T R;
+    struct Row { typename Raw<DT, VE>::T v; float w; };
     const uint32_t lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
-    const uint32_t v0 = blockIdx.x * (U * kWave) + lane;
-    struct Row { R v[U]; float w; };
+    const Place<DT, VE> p(blockIdx.x * kWave + lane, a.nvec, a.dim);
     for (uint64_t token = (uint64_t)blockIdx.y * kMoveWaves + wave; token < a.tokens; token += (uint64_t)gridDim.y * kMoveWaves) {
         const uint64_t slot = token * a.topk + min(lane, a.topk - 1);
         const uint32_t listed = (uint32_t)a.row_of_slot[slot];
         float weight = 1.f;
         if (a.weights) weight = load_one<DT>(a.weights, a.weights_f32, slot);
-        float sum[U][VE] = {};
+        float sum[VE] = {};
         uint64_t left = __ballot(lane < a.topk && listed < a.nrows);
         in_batches<8>((uint32_t)__popcll(left),
-                   [&](uint32_t) {
-                       const int k = __builtin_ctzll(left);
-                       left &= left - 1;
-                       const char* const from = a.in + (uint64_t)lane_value(listed, k) * a.row_bytes;
-                       Row r;
-                       r.w = lane_value(weight, k);
+                      [&](uint32_t) {
+                          const int k = __builtin_ctzll(left);
+                          left &= left - 1;
+                          return Row{load<DT, VE, NT>(a.in + (uint64_t)lane_value(listed, k) * a.row_bytes, p.byte()), lane_value(weight, k)};
+                      },
+                      [&](const Row& r) {
+                          float x[VE];
+                          unpack<DT, VE>(r.v, x);
 #pragma unroll
-                       for (int u = 0; u < U; ++u) r.v[u] = load<DT, VE, NT>(from, Place<DT, VE>(v0 + u * kWave, a.nvec, a.dim).byte());
-                       return r;
-                   },
-                   [&](const Row& r) {
-#pragma unroll
-                       for (int u = 0; u < U; ++u) {
-                           float x[VE];
-                           unpack<DT, VE>(r.v[u], x);
-#pragma unroll
-                           for (int i = 0; i < VE; ++i) sum[u][i] = fmaf(r.w, x[i], sum[u][i]);
-                       }
-                   });
-        char* const to = a.out + token * a.row_bytes;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const Place<DT, VE> p(v0 + u * kWave, a.nvec, a.dim);
-            if (p.in) store<DT, VE, NT>(to, p.byte(), pack<DT, VE>(sum[u]));
-        }
+                          for (int i = 0; i < VE; ++i) sum[i] = fmaf(r.w, x[i], sum[i]);
+                      });
+        if (p.in) store<DT, VE, NT>(a.out + token * a.row_bytes, p.byte(), pack<DT, VE>(sum));
     }
 }
 
 // Both gradients in one pass over the rows: a token's gradient row stays in registers while its rows go by, each read
 // once for its dot product (summed in 32 bits, kept in the lane of its choice) and written once.  SHARE waves take one
-// token's segments in turn where the rows are long; their dot products are added in wave order.
+// token's segments in turn where the rows are long; their dot products are added in wave order.  Bound by HBM: 16384
+// tokens of 4096 in bf16, four choices (1.2 GB) 222 us, 5.4 TB/s.
 template <int DT, int VE, int U, int SHARE, bool NT>
 __global__ __launch_bounds__(kMoveThreads) void combine_backward_kernel(const MoveArgs a) {
     typedef typename Raw<DT, VE>::T R;
@@ -583,7 +570,10 @@ __global__ __launch_bounds__(kMoveThreads) void combine_backward_kernel(const Mo
 }
 
 // ---- sum over the ranks, norms, gate, residual ----------------------------------------------------------------
-// A workgroup takes one token; its row stays in registers in 32 bits from the sum over the ranks to the last norm.
+// A workgroup takes one token; its row stays in registers in 32 bits from the sum over the ranks to the last norm, one
+// 16-byte vector a thread as long as 1024 threads reach (two at 4096 columns: 228 us against 220 for eight ranks' 8192
+// tokens, 6.3 against 5.4 for eight tokens).  Bound by HBM: those 8192 tokens of 4096 in bf16 with a copy of the result for
+// every rank (1.2 GB) 205 us, 5.9 TB/s.  A grid that stays and keeps its weights in registers was slower (240).
 struct NormArgs {
     const char* partials[SAR_MAX_RANKS];
     const char* residual;
@@ -753,6 +743,9 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_kernel(const NormArg
 // hidden is computed again from y and the residual, so nothing that was rounded comes back.  A workgroup walks over
 // tokens and keeps the column sums in registers; they leave as one row of sums per workgroup, added up by
 // column_sum_kernel in a fixed order; a single workgroup writes the gradients itself.
+// Bound by HBM where ranks are many: 4096 tokens of 4096 in bf16 to and from eight ranks (0.87 GB) 135 us, 6.4 TB/s; by the
+// two sums over a row that every token waits for where they are not: one row in, one out 53 us for 0.23 GB.  Loading the next
+// token ahead cost registers that were spilled (79 us), as did five or six waves a SIMD (71, 93).
 struct NormBackwardArgs {
     NormArgs f;
     const char* total;
@@ -1104,39 +1097,30 @@ template <class F> void with_bool(bool b, F&& f) {
     else f(std::false_type{});
 }
 
-// Vectors per lane: several where that still leaves every CU its waves, one where there are few tokens (the smallest
-// calls are bound by the time of one trip to memory, and more waves make it one trip instead of four).
-bool many_vectors(const MoveArgs& a, uint32_t u) {
-    const uint64_t segments = (a.nvec + u * kWave - 1) / (u * kWave);
-    return a.tokens * segments >= 4096 && a.nvec > kWave;
-}
-
-dim3 move_grid(const MoveArgs& a, int u) {
+// One vector a lane: two and four were level for the large calls (16384 tokens of 2048, eight choices: combine 101 us with
+// two, 101 with one; dispatch with its gradient 212 with four, 219 with two, 210 with one) and slower for the small ones (32
+// tokens: 3.9 us with four, 3.1) and for rows that do not fill them (3000 of 7168: 73 with four, 64).
+dim3 move_grid(const MoveArgs& a) {
     const uint64_t groups = (a.tokens + kMoveWaves - 1) / kMoveWaves;
-    return dim3((a.nvec + u * kWave - 1) / (u * kWave), (uint32_t)std::min<uint64_t>(groups, 65535u));
+    return dim3((a.nvec + kWave - 1) / kWave, (uint32_t)std::min<uint64_t>(groups, 65535u));
 }
 
-constexpr int kDispatchVectors = 4, kCombineVectors = 2;
+// calls f(integral_constant<int, VE>, integral_constant<bool, NT>) for a call
+template <int DT, class F> void with_move_shape(const MoveArgs& a, F&& f) {
+    if (a.dim < kVec<DT>) f(std::integral_constant<int, 1>{}, std::false_type{});
+    else with_bool(((uint64_t)a.nrows + a.tokens) * a.row_bytes >= kStreamBytes, [&](auto nt) { f(std::integral_constant<int, kVec<DT>>{}, nt); });
+}
 
 template <int DT> void launch_dispatch(hipStream_t st, const MoveArgs& a) {
-    const bool nt = ((uint64_t)a.nrows + a.tokens) * a.row_bytes >= kStreamBytes;
     with_bool(a.weights != nullptr, [&](auto weighted) {
-        constexpr bool W = decltype(weighted)::value;
-        constexpr int U = kDispatchVectors;
-        if (a.dim < kVec<DT>) dispatch_kernel<DT, 1, 1, false, W><<<move_grid(a, 1), kMoveThreads, 0, st>>>(a);
-        else if (!many_vectors(a, U)) dispatch_kernel<DT, kVec<DT>, 1, false, W><<<move_grid(a, 1), kMoveThreads, 0, st>>>(a);
-        else if (nt) dispatch_kernel<DT, kVec<DT>, U, true, W><<<move_grid(a, U), kMoveThreads, 0, st>>>(a);
-        else dispatch_kernel<DT, kVec<DT>, U, false, W><<<move_grid(a, U), kMoveThreads, 0, st>>>(a);
+        with_move_shape<DT>(a, [&](auto ve, auto nt) {
+            dispatch_kernel<DT, decltype(ve)::value, decltype(nt)::value, decltype(weighted)::value><<<move_grid(a), kMoveThreads, 0, st>>>(a);
+        });
     });
 }
 
 template <int DT> void launch_combine(hipStream_t st, const MoveArgs& a) {
-    const bool nt = ((uint64_t)a.nrows + a.tokens) * a.row_bytes >= kStreamBytes;
-    constexpr int U = kCombineVectors;
-    if (a.dim < kVec<DT>) combine_kernel<DT, 1, 1, false><<<move_grid(a, 1), kMoveThreads, 0, st>>>(a);
-    else if (!many_vectors(a, U)) combine_kernel<DT, kVec<DT>, 1, false><<<move_grid(a, 1), kMoveThreads, 0, st>>>(a);
-    else if (nt) combine_kernel<DT, kVec<DT>, U, true><<<move_grid(a, U), kMoveThreads, 0, st>>>(a);
-    else combine_kernel<DT, kVec<DT>, U, false><<<move_grid(a, U), kMoveThreads, 0, st>>>(a);
+    with_move_shape<DT>(a, [&](auto ve, auto nt) { combine_kernel<DT, decltype(ve)::value, decltype(nt)::value><<<move_grid(a), kMoveThreads, 0, st>>>(a); });
 }
 
 // A wave takes a token, with as many vectors a lane as the row has; four waves share one where the row is longer than
