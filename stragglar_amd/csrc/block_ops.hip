@@ -743,7 +743,7 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_kernel(const NormArg
 // hidden is computed again from y and the residual, so nothing that was rounded comes back.  A workgroup walks over
 // tokens and keeps the column sums in registers; they leave as one row of sums per workgroup, added up by
 // column_sum_kernel in a fixed order; a single workgroup writes the gradients itself.
-// Bound by HBM where ranks are many: 4096 tokens of 4096 in bf16 to and from eight ranks (0.87 GB) 135 us, 6.4 TB/s; by the
+// Bound by HBM where ranks are many: 4096 tokens of 4096 in bf16 to and from eight ranks (0.73 GB) 133 us, 5.5 TB/s; by the
 // two sums over a row that every token waits for where they are not: one row in, one out 53 us for 0.23 GB.  Loading the next
 // token ahead cost registers that were spilled (79 us), as did five or six waves a SIMD (71, 93).
 struct NormBackwardArgs {
