@@ -1342,7 +1342,7 @@ int sar_combine_backward(int device, void* stream, int dtype, const void* grad, 
         a.rows = (const char*)rows;
         a.out = (char*)grad_rows;
         a.grad_weights = (char*)grad_weights;
-        a.total = offsets + num_experts;
+        a.total = offsets ? offsets + num_experts : nullptr;
         with_dtype(dtype, [&](auto dt) { launch_combine_backward<decltype(dt)::value>((hipStream_t)stream, a); });
         return launched("sar_combine_backward");
     });

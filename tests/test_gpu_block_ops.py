@@ -669,6 +669,48 @@ def test_on_another_stream(groups):
     assert torch.equal(got, want)
 
 
+def test_two_streams_at_once(groups):
+    """Calls of different sizes on two streams, one after the other without waiting: nothing is shared between them."""
+    g = groups(4)
+    jobs = []
+    for i, (t, d) in enumerate([(9000, 264), (700, 1001)]):
+        e, x, res = choices(i, t, 4, 16, 0.1), randn(10 + i, t, d), randn(20 + i, t, d)
+        w, gw, gh = randn(30 + i, d, mean=1.0, scale=0.1), torch.softmax(randn(40 + i, t, 4), 1), randn(50 + i, t, d)
+        jobs.append((e, x, res, w, gw, gh))
+
+    def work(e, x, res, w, gw, gh):
+        with torch.no_grad():
+            r = g.route(e, 16)
+            y = g.combine(g.dispatch(x, r), r, gw)
+            h, n, saved = g.reduce_norm([x, y, x, y], res, pre_weight=w, post_weight=w, gate=w, save=True)
+            return [y, h, n, *g.reduce_norm_backward(saved, gh, n), *g.combine_backward(gh, g.dispatch(x, r), r, gw)]
+    want = [work(*j) for j in jobs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(work(*jobs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[i])), i
+
+
+def test_no_tokens(groups):
+    g = groups(4)
+    r = g.route(torch.zeros(0, 2, dtype=torch.int64, device="cuda"), 8)
+    assert r.offsets.tolist() == [0] * 9 and r.slot_of_row.numel() == 0
+    x, w = torch.zeros(0, 16, device="cuda", requires_grad=True), torch.zeros(0, 2, device="cuda", requires_grad=True)
+    rows = g.dispatch(x, r)
+    y = g.combine(rows, r, w)
+    assert rows.shape == (0, 16) and y.shape == (0, 16)
+    gx, gw = torch.autograd.grad(y.sum(), (x, w))
+    assert gx.shape == (0, 16) and gw.shape == (0, 2)
+
+
 def test_captured_and_replayed(groups):
     """Forward and explicit backward in two graphs, replayed in turn with eager work in between, on changing inputs."""
     g, n, t, d, e, k = groups(4), 4, 700, 136, 16, 4
