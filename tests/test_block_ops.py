@@ -102,6 +102,23 @@ def test_reduce_norm_backward_refuses(group):
             call()
 
 
+def test_a_capturing_stream_refuses_autograd(monkeypatch):
+    """Neither the recording nor the backward pass of a recorded call goes into a capture; without gradients the check
+    is not even made."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    x = torch.zeros(2, 2, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        block_ops._recording(None, x)
+    with torch.no_grad():
+        assert not block_ops._recording(x)
+    assert not block_ops._recording(x.detach(), None)
+    for node in (block_ops._Dispatch, block_ops._Combine, block_ops._ReduceNorm):
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            node._backward(None, x)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert block_ops._recording(x)
+
+
 def refused(lib, rc, why):
     assert rc == -1 and why in lib.lib.sar_last_error().decode(), (rc, lib.lib.sar_last_error())
 
