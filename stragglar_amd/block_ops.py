@@ -250,23 +250,38 @@ def _routing_rows(group, name, t, routing, sorted_rows):
         raise ValueError("%s needs 1 to 2^24 columns" % name)
 
 
+def _fits_rows(group, t, routing, sorted_rows):
+    """Whether the checks above and of the device pass, in as little time as they take."""
+    if not isinstance(t, torch.Tensor) or not isinstance(routing, Routing) or t.dim() != 2:
+        return False
+    tokens, topk = routing.row_of_slot.shape
+    return (t.shape[0] == (tokens * topk if sorted_rows else tokens) and t.dtype in DTYPE_CODES and t.is_contiguous()
+            and t.get_device() == group.device and routing.offsets.get_device() == group.device and 1 <= t.shape[1] <= 1 << 24)
+
+
 def _check_weights(routing, weights, dtype):
     if weights is not None:
         _tensor("weights", weights, routing.row_of_slot.shape, (torch.float32, dtype))
 
 
 def dispatch(group, tokens, routing):
-    _routing_rows(group, "tokens", tokens, routing, False)
-    _on_device(group, tokens=tokens, routing=routing.offsets)
+    if not _fits_rows(group, tokens, routing, False):
+        _routing_rows(group, "tokens", tokens, routing, False)
+        _on_device(group, tokens=tokens, routing=routing.offsets)
     if _recording(tokens):
         return _Dispatch.apply(tokens, (group, routing))
     return _dispatch(group, tokens, routing)
 
 
 def combine(group, rows, routing, weights=None):
-    _routing_rows(group, "rows", rows, routing, True)
-    _check_weights(routing, weights, rows.dtype)
-    _on_device(group, rows=rows, weights=weights, routing=routing.offsets)
+    if not _fits_rows(group, rows, routing, True):
+        _routing_rows(group, "rows", rows, routing, True)
+        _check_weights(routing, weights, rows.dtype)
+        _on_device(group, rows=rows, weights=weights, routing=routing.offsets)
+    if weights is not None:
+        _check_weights(routing, weights, rows.dtype)
+        if weights.get_device() != group.device:
+            _on_device(group, weights=weights)
     if _recording(rows, weights):
         return _Combine.apply(rows, weights, (group, routing))
     return _combine(group, rows, routing, weights)
@@ -312,25 +327,25 @@ def _norm_args(sources, copies, residual, pre_weight, post_weight, gate, residua
                                residual.data_ptr(), pre, post, gate_ptr, hidden, normed, total, stats)
 
 
-def _reduce_norm(group, partials, residual, pre_weight, post_weight, gate, residual_scale, eps, gather, save):
-    """`partials`: sequence of tensors [tokens, dim], or one tensor [n, tokens, dim].  Returns hidden, normed (or None),
-    total and stats (or None)."""
+@functools.lru_cache(maxsize=None)
+def _pointers(n):
+    return ctypes.c_void_p * n
+
+
+def _reduce_norm(group, partials, addresses, residual, pre_weight, post_weight, gate, residual_scale, eps, gather, save):
+    """`addresses`: of the partials' rows.  Returns hidden, normed (or None), total and stats (or None); one partial is
+    its own total."""
     tokens, dim = residual.shape
-    if isinstance(partials, torch.Tensor):
-        step, base = tokens * dim * residual.element_size(), partials.data_ptr()
-        addresses = [base + r * step for r in range(partials.shape[0])]
-    else:
-        addresses = [p.data_ptr() for p in partials]
     sources = len(addresses)
     hidden = torch.empty_like(residual)
     normed = total = stats = None
     if pre_weight is not None:
         normed = residual.new_empty((group.n, tokens, dim) if gather else (tokens, dim))
     if save:
-        total = partials[0] if sources == 1 else torch.empty((tokens, dim), dtype=torch.float32, device=residual.device)
+        total = partials if sources == 1 else torch.empty((tokens, dim), dtype=torch.float32, device=residual.device)
         stats = torch.empty((2, tokens), dtype=torch.float32, device=residual.device)
     args = _norm_args(sources, group.n if gather else 1, residual, pre_weight, post_weight, gate, residual_scale, eps,
-                      (ctypes.c_void_p * sources)(*addresses), hidden.data_ptr(), _ptr(normed),
+                      _pointers(sources)(*addresses), hidden.data_ptr(), _ptr(normed),
                       total.data_ptr() if save and sources > 1 else None, _ptr(stats))
     lib = group._lib
     lib.check(lib.lib.sar_reduce_norm(group.device, _raw_stream(group.device), ctypes.byref(args)))
@@ -361,9 +376,9 @@ def _reduce_norm_backward(group, s: ReduceNormSaved, grad_hidden, grad_normed, w
 class _ReduceNorm(_Node):
     @staticmethod
     def forward(ctx, plain, residual, pre_weight, post_weight, gate, *partials):
-        group, shape, residual_scale, eps, gather = plain
-        rows = partials[0] if len(shape) == 3 and len(partials) == 1 else partials
-        hidden, normed, total, stats = _reduce_norm(group, rows, residual, pre_weight, post_weight, gate, residual_scale, eps, gather, True)
+        group, shape, addresses, residual_scale, eps, gather = plain
+        hidden, normed, total, stats = _reduce_norm(group, partials[0], addresses, residual, pre_weight, post_weight, gate, residual_scale, eps,
+                                                    gather, True)
         ctx.plain = plain
         ctx.save_for_backward(total, stats, residual, pre_weight, post_weight, gate)
         ctx.set_materialize_grads(False)
@@ -372,8 +387,8 @@ class _ReduceNorm(_Node):
     @staticmethod
     def gradients(ctx, grad_hidden, grad_normed):
         total, stats, residual, pre_weight, post_weight, gate = ctx.saved_tensors
-        group, shape, residual_scale, eps, gather = ctx.plain
-        saved = ReduceNormSaved(group.n if len(shape) == 3 else 1, group.n if gather else 1, shape, total, stats, residual, pre_weight,
+        group, shape, addresses, residual_scale, eps, gather = ctx.plain
+        saved = ReduceNormSaved(len(addresses), group.n if gather else 1, shape, total, stats, residual, pre_weight,
                                 post_weight, gate, residual_scale, eps)
         need = ctx.needs_input_grad
         g = _reduce_norm_backward(group, saved, grad_hidden.contiguous() if grad_hidden is not None else None,
@@ -423,48 +438,52 @@ def _check_reduce_norm(group, partials, inputs, residual, pre_weight, post_weigh
 
 
 def _fits_reduce_norm(group, partials, inputs, residual, pre_weight, post_weight, gate, eps):
-    """The checks above in as little time as they take."""
+    """The checks above in as little time as they take: the addresses of the partials' rows, or None."""
     if not isinstance(residual, torch.Tensor) or residual.dim() != 2:
-        return False
+        return None
     size, dtype, device = residual.shape, residual.dtype, group.device
-    dim = size[1]
+    tokens, dim = size
     if dtype not in DTYPE_CODES or not 1 <= dim <= MAX_NORM_DIM or not residual.is_contiguous() or residual.get_device() != device or not 0 <= eps < float("inf"):
-        return False
-    if isinstance(partials, torch.Tensor):
-        if partials.shape != size and partials.shape != (group.n, *size):
-            return False
-        size = partials.shape
-    elif len(inputs) != group.n:
-        return False
+        return None
+    whole = partials is inputs[0] and partials.dim() == 3
+    if whole:
+        size = (group.n, tokens, dim)
+    elif partials is not inputs[0] and len(inputs) != group.n:
+        return None
+    addresses = []
     for p in inputs:
         if not isinstance(p, torch.Tensor) or p.dtype is not dtype or p.shape != size or not p.is_contiguous() or p.get_device() != device:
-            return False
+            return None
+        addresses.append(p.data_ptr())
+    if whole:
+        addresses = [addresses[0] + r * tokens * dim * residual.element_size() for r in range(group.n)]
     for w in (pre_weight, post_weight):
         if w is not None and (not isinstance(w, torch.Tensor) or w.dim() != 1 or w.shape[0] != dim or not w.is_contiguous() or w.get_device() != device
                               or (w.dtype is not dtype and w.dtype is not torch.float32)):
-            return False
-    return gate is None or (isinstance(gate, torch.Tensor) and gate.is_contiguous() and gate.get_device() == device
-                            and (gate.dtype is dtype or gate.dtype is torch.float32)
-                            and tuple(gate.shape) in ((dim,), (residual.shape[0], 1), (residual.shape[0], dim)))
+            return None
+    if gate is not None and not (isinstance(gate, torch.Tensor) and gate.is_contiguous() and gate.get_device() == device
+                                 and (gate.dtype is dtype or gate.dtype is torch.float32) and tuple(gate.shape) in ((dim,), (tokens, 1), (tokens, dim))):
+        return None
+    return addresses
 
 
 def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], residual, pre_weight=None, post_weight=None, gate=None,
                 residual_scale: float = 1.0, eps: float = 1e-6, gather: bool = True, save: bool = False):
     inputs = (partials,) if isinstance(partials, torch.Tensor) else tuple(partials)
-    if not _fits_reduce_norm(group, partials, inputs, residual, pre_weight, post_weight, gate, eps):
+    addresses = _fits_reduce_norm(group, partials, inputs, residual, pre_weight, post_weight, gate, eps) if inputs else None
+    if addresses is None:
         _check_reduce_norm(group, partials, inputs, residual, pre_weight, post_weight, gate, eps)
         raise ValueError("the arguments do not fit each other")
     shape = tuple(partials.shape) if inputs[0] is partials else (group.n, *residual.shape)
     if _recording(residual, pre_weight, post_weight, gate, *inputs):
         if save:
             raise ValueError("save=True is for calls under torch.no_grad(): autograd keeps what it needs by itself")
-        return _ReduceNorm.apply((group, shape, residual_scale, eps, gather), residual, pre_weight, post_weight, gate, *inputs)
-    rows = partials if len(shape) == 3 and len(inputs) == 1 else inputs
-    hidden, normed, total, stats = _reduce_norm(group, rows, residual, pre_weight, post_weight, gate, residual_scale, eps, gather, save)
+        return _ReduceNorm.apply((group, shape, addresses, residual_scale, eps, gather), residual, pre_weight, post_weight, gate, *inputs)
+    hidden, normed, total, stats = _reduce_norm(group, inputs[0], addresses, residual, pre_weight, post_weight, gate, residual_scale, eps, gather, save)
     if not save:
         return hidden, normed
-    return hidden, normed, ReduceNormSaved(group.n if len(shape) == 3 else 1, group.n if gather else 1, shape, total, stats, residual,
-                                           pre_weight, post_weight, gate, residual_scale, eps)
+    return hidden, normed, ReduceNormSaved(len(addresses), group.n if gather else 1, shape, total, stats, residual, pre_weight, post_weight, gate,
+                                           residual_scale, eps)
 
 
 def reduce_norm_backward(group, saved: ReduceNormSaved, grad_hidden=None, grad_normed=None) -> ReduceNormGrads:
