@@ -28,7 +28,8 @@ class Routing:
     """Where every (token, choice) slot goes, as ``EmulatedGroup.route`` found it.  ``row_of_slot`` [tokens, topk]: the
     slot's row among the rows sorted by expert, -1 = dropped.  ``slot_of_row`` [tokens * topk]: the slot (token * topk
     + choice) of each row, -1 behind the last.  ``offsets`` [num_experts + 1]: first row of each expert, then the
-    number of rows; ``rank_offsets`` [ranks + 1]: the same for the ranks that own the experts.  All int32 on the GPU."""
+    number of rows; ``rank_offsets`` [ranks + 1]: the same for the ranks that own the experts.  All int32 on the GPU.  The tensors
+    stay as they are until the backward pass of every call that took them has run; autograd raises if they did not."""
 
     __slots__ = ("row_of_slot", "slot_of_row", "offsets", "num_experts", "ranks")
 
@@ -169,49 +170,57 @@ def route(group, experts, num_experts: int) -> Routing:
 
 # ---- dispatch, combine -----------------------------------------------------------------------------------------
 
-def _dispatch(group, rows, routing, weights=None):
-    tokens, topk = routing.row_of_slot.shape
+def _dispatch(group, rows, row_of_slot, offsets, weights=None):
+    tokens, topk = row_of_slot.shape
     dim = rows.shape[1]
     out = rows.new_empty((tokens * topk, dim))
-    lib = group._lib
-    lib.check(lib.lib.sar_dispatch(group.device, _raw_stream(group.device), DTYPE_CODES[rows.dtype], rows.data_ptr(), tokens, topk, dim,
-                                   routing.row_of_slot.data_ptr(), routing.offsets.data_ptr(), routing.num_experts,
+    code, lib = DTYPE_CODES[rows.dtype], group._lib
+    lib.check(lib.lib.sar_dispatch(group.device, _raw_stream(group.device), code, rows.data_ptr(), tokens, topk, dim,
+                                   row_of_slot.data_ptr(), offsets.data_ptr(), offsets.numel() - 1,
                                    _ptr(weights), DTYPE_CODES[weights.dtype] if weights is not None else 0, out.data_ptr()))
     return out
 
 
-def _combine(group, rows, routing, weights=None):
-    tokens, topk = routing.row_of_slot.shape
+def _combine(group, rows, row_of_slot, weights=None):
+    tokens, topk = row_of_slot.shape
     dim = rows.shape[1]
     out = rows.new_empty((tokens, dim))
-    lib = group._lib
-    lib.check(lib.lib.sar_combine(group.device, _raw_stream(group.device), DTYPE_CODES[rows.dtype], rows.data_ptr(), tokens, topk, dim,
-                                  routing.row_of_slot.data_ptr(), _ptr(weights), DTYPE_CODES[weights.dtype] if weights is not None else 0, out.data_ptr()))
+    code, lib = DTYPE_CODES[rows.dtype], group._lib
+    lib.check(lib.lib.sar_combine(group.device, _raw_stream(group.device), code, rows.data_ptr(), tokens, topk, dim,
+                                  row_of_slot.data_ptr(), _ptr(weights), DTYPE_CODES[weights.dtype] if weights is not None else 0, out.data_ptr()))
     return out
 
 
-def _combine_backward(group, grad, rows, routing, weights, want_rows, want_weights):
+def _combine_backward(group, grad, rows, row_of_slot, offsets, weights, want_rows, want_weights):
     if not want_weights:
-        return (_dispatch(group, grad, routing, weights) if want_rows else None), None
-    tokens, topk = routing.row_of_slot.shape
+        return (_dispatch(group, grad, row_of_slot, offsets, weights) if want_rows else None), None
+    tokens, topk = row_of_slot.shape
     grad_rows = torch.empty_like(rows) if want_rows else None
     grad_weights = torch.empty_like(weights)
     lib = group._lib
     lib.check(lib.lib.sar_combine_backward(group.device, _raw_stream(group.device), DTYPE_CODES[rows.dtype], grad.data_ptr(), rows.data_ptr(),
-                                           tokens, topk, rows.shape[1], routing.row_of_slot.data_ptr(), routing.offsets.data_ptr(),
-                                           routing.num_experts, weights.data_ptr(), DTYPE_CODES[weights.dtype], _ptr(grad_rows), grad_weights.data_ptr()))
+                                           tokens, topk, rows.shape[1], row_of_slot.data_ptr(), offsets.data_ptr(), offsets.numel() - 1,
+                                           weights.data_ptr(), DTYPE_CODES[weights.dtype], _ptr(grad_rows), grad_weights.data_ptr()))
     return grad_rows, grad_weights
+
+
+def _savable(t):
+    """A routing's tensor for save_for_backward, whose version autograd then holds against the one it finds in the
+    backward pass.  What route() made under inference_mode has no version and is refused there: a copy has one."""
+    return t.clone() if t.is_inference() else t
 
 
 class _Dispatch(_Node):
     @staticmethod
     def forward(ctx, rows, plain):
-        ctx.plain = plain
-        return _dispatch(plain[0], rows, plain[1])
+        group, routing = plain
+        ctx.group = group
+        ctx.save_for_backward(_savable(routing.row_of_slot))
+        return _dispatch(group, rows, routing.row_of_slot, routing.offsets)
 
     @staticmethod
     def gradients(ctx, grad):
-        return _combine(ctx.plain[0], grad.contiguous(), ctx.plain[1]), None
+        return _combine(ctx.group, grad.contiguous(), ctx.saved_tensors[0]), None
 
     @staticmethod
     def backward(ctx, grad):
@@ -221,15 +230,16 @@ class _Dispatch(_Node):
 class _Combine(_Node):
     @staticmethod
     def forward(ctx, rows, weights, plain):
-        ctx.plain = plain
-        ctx.save_for_backward(rows, weights)
-        return _combine(plain[0], rows, plain[1], weights)
+        group, routing = plain
+        ctx.group = group
+        ctx.save_for_backward(rows, weights, _savable(routing.row_of_slot), _savable(routing.offsets))
+        return _combine(group, rows, routing.row_of_slot, weights)
 
     @staticmethod
     def gradients(ctx, grad):
-        rows, weights = ctx.saved_tensors
+        rows, weights, row_of_slot, offsets = ctx.saved_tensors
         need = ctx.needs_input_grad
-        a, b = _combine_backward(ctx.plain[0], grad.contiguous(), rows, ctx.plain[1], weights, need[0], weights is not None and need[1])
+        a, b = _combine_backward(ctx.group, grad.contiguous(), rows, row_of_slot, offsets, weights, need[0], weights is not None and need[1])
         return a, b, None
 
     @staticmethod
@@ -270,7 +280,7 @@ def dispatch(group, tokens, routing):
         _on_device(group, tokens=tokens, routing=routing.offsets)
     if _recording(tokens):
         return _Dispatch.apply(tokens, (group, routing))
-    return _dispatch(group, tokens, routing)
+    return _dispatch(group, tokens, routing.row_of_slot, routing.offsets)
 
 
 def combine(group, rows, routing, weights=None):
@@ -284,13 +294,13 @@ def combine(group, rows, routing, weights=None):
             _on_device(group, weights=weights)
     if _recording(rows, weights):
         return _Combine.apply(rows, weights, (group, routing))
-    return _combine(group, rows, routing, weights)
+    return _combine(group, rows, routing.row_of_slot, weights)
 
 
 def dispatch_backward(group, grad, routing):
     _routing_rows(group, "grad", grad, routing, True)
     _on_device(group, grad=grad, routing=routing.offsets)
-    return _combine(group, grad, routing)
+    return _combine(group, grad, routing.row_of_slot)
 
 
 def combine_backward(group, grad, rows, routing, weights=None):
@@ -298,7 +308,7 @@ def combine_backward(group, grad, rows, routing, weights=None):
     _tensor("grad", grad, (routing.tokens, rows.shape[1]), (rows.dtype,))
     _check_weights(routing, weights, rows.dtype)
     _on_device(group, grad=grad, rows=rows, weights=weights, routing=routing.offsets)
-    return _combine_backward(group, grad, rows, routing, weights, True, weights is not None)
+    return _combine_backward(group, grad, rows, routing.row_of_slot, routing.offsets, weights, True, weights is not None)
 
 
 # ---- sum over the ranks, norms, gate, residual -------------------------------------------------------------------

@@ -204,3 +204,52 @@ def test_struct_sizes_follow_the_header(tmp_path):
     got = [int(x) for x in subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.split()]
     assert got == [ctypes.sizeof(capi.ReduceNormArgs), capi.ReduceNormArgs.stats.offset,
                    ctypes.sizeof(capi.ReduceNormGrads), capi.ReduceNormGrads.workspace_bytes.offset]
+
+
+# ---- calls that get past the checks: on the CPU, with nothing behind the C entries ---------------------------------
+
+@pytest.fixture()
+def recorder(monkeypatch):
+    """A group whose tensors lie on the CPU and whose C entries only note their names in `calls`."""
+    class Entries:
+        def __getattr__(self, name):
+            return lambda *args: g.calls.append(name) or 0
+
+    class Lib:
+        lib = Entries()
+
+        def check(self, rc):
+            assert rc == 0
+    g = object.__new__(EmulatedGroup)
+    g.n, g.device, g._lib, g.calls = 4, -1, Lib(), []
+    monkeypatch.setattr(block_ops, "_raw_stream", lambda device: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return g
+
+
+def test_a_routing_written_again_is_noticed_by_the_backward_pass(recorder):
+    g = recorder
+    for field in ("row_of_slot", "offsets"):
+        r = routing()
+        x, rows = torch.zeros(3, 8, requires_grad=True), torch.zeros(6, 8, requires_grad=True)
+        w = torch.zeros(3, 2, requires_grad=True)
+        outs = [(g.combine(rows, r, w), (rows, w)), (g.combine(rows, r), (rows,))]
+        if field == "row_of_slot":                        # (what dispatch's gradient reads)
+            outs.append((g.dispatch(x, r), (x,)))
+        getattr(r, field).copy_(torch.ones_like(getattr(r, field)))
+        g.calls.clear()
+        for out, leaves in outs:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(out.sum(), leaves)
+        assert not g.calls
+    r = routing()                                          # left alone, it is what the backward pass gets
+    torch.autograd.grad(g.combine(rows, r, w).sum(), (rows, w))
+    assert g.calls == ["sar_combine", "sar_combine_backward"]
+
+
+def test_a_routing_made_in_inference_mode_takes_part_in_autograd(recorder):
+    with torch.inference_mode():
+        r = routing()
+    x, rows = torch.zeros(3, 8, requires_grad=True), torch.zeros(6, 8, requires_grad=True)
+    assert torch.autograd.grad(recorder.dispatch(x, r).sum(), x)[0].shape == (3, 8)
+    assert torch.autograd.grad(recorder.combine(rows, r).sum(), rows)[0].shape == (6, 8)

@@ -805,3 +805,24 @@ def test_offsets_beyond_32_bits(groups):
         part = rows[a:a + 20]
         h, x, want = plain_norm(dict(s, partials=part, residual=part), 1.0, 1e-6, part, normed[a:a + 20].unsqueeze(0))
         check(hidden[a:a + 20], h, a), check(normed[a:a + 20], x, a), check(back.residual[a:a + 20], want["residual"], a)
+
+
+def test_a_routing_between_forward_and_backward(groups):
+    """Written again in place it is refused; what route() made under inference_mode gives the gradients of any other."""
+    g, t, k, d = groups(4), 50, 2, 40
+    e = choices(1, t, k, 8, 0.2)
+    x, rows = randn(2, t, d).requires_grad_(True), randn(3, t * k, d).requires_grad_(True)
+    w, gx, gr = randn(4, t, k).requires_grad_(True), randn(5, t * k, d), randn(6, t, d)
+
+    def forward(r):
+        return (g.dispatch(x, r), g.combine(rows, r, w)), (x, rows, w), (gx, gr)
+    r = g.route(e, 8)
+    want = torch.autograd.grad(*forward(r))
+    with torch.inference_mode():
+        made = g.route(e, 8)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(*forward(made)), want))
+    for outs in ((g.dispatch(x, r),), (g.combine(rows, r, w),), (g.combine(rows, r),)):
+        again = g.route(choices(7, t, k, 8, 0.2), 8)
+        r.row_of_slot.copy_(again.row_of_slot), r.offsets.copy_(again.offsets)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            outs[0].sum().backward()
