@@ -16,6 +16,7 @@ import functools
 from typing import NamedTuple, Optional, Sequence, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import capi
 
@@ -105,8 +106,18 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+def _refuse_tangents(*tensors):
+    """There are no forward-mode derivatives: a tangent would be lost, which reads as a derivative of zero."""
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("the block operators have no forward-mode derivatives")
+
+
 def _recording(*tensors) -> bool:
     """Whether autograd has to record the call."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(*tensors)
     if not torch.is_grad_enabled():
         return False
     for t in tensors:
@@ -300,6 +311,7 @@ def combine(group, rows, routing, weights=None):
 def dispatch_backward(group, grad, routing):
     _routing_rows(group, "grad", grad, routing, True)
     _on_device(group, grad=grad, routing=routing.offsets)
+    _refuse_tangents(grad)
     return _combine(group, grad, routing.row_of_slot)
 
 
@@ -308,6 +320,7 @@ def combine_backward(group, grad, rows, routing, weights=None):
     _tensor("grad", grad, (routing.tokens, rows.shape[1]), (rows.dtype,))
     _check_weights(routing, weights, rows.dtype)
     _on_device(group, grad=grad, rows=rows, weights=weights, routing=routing.offsets)
+    _refuse_tangents(grad, rows, weights)
     return _combine_backward(group, grad, rows, routing.row_of_slot, routing.offsets, weights, True, weights is not None)
 
 
@@ -510,4 +523,5 @@ def reduce_norm_backward(group, saved: ReduceNormSaved, grad_hidden=None, grad_n
             raise ValueError("grad_normed has shape %s, need %s" % (tuple(grad_normed.shape), ok[-1]))
         _tensor("grad_normed", grad_normed, dtypes=(saved.residual.dtype,))
     _on_device(group, grad_hidden=grad_hidden, grad_normed=grad_normed, residual=saved.residual)
+    _refuse_tangents(grad_hidden, grad_normed, saved.total, saved.residual, saved.pre_weight, saved.post_weight, saved.gate)
     return _reduce_norm_backward(group, saved, grad_hidden, grad_normed, (True,) * 5)

@@ -253,3 +253,45 @@ def test_a_routing_made_in_inference_mode_takes_part_in_autograd(recorder):
     x, rows = torch.zeros(3, 8, requires_grad=True), torch.zeros(6, 8, requires_grad=True)
     assert torch.autograd.grad(recorder.dispatch(x, r).sum(), x)[0].shape == (3, 8)
     assert torch.autograd.grad(recorder.combine(rows, r).sum(), rows)[0].shape == (6, 8)
+
+
+def every_call(g, r, make=lambda t: t):
+    """One call of each kind per floating-point input, that input passed through `make`: (name, call)."""
+    t, k, d = 3, 2, 8
+    z = lambda *shape: torch.zeros(*shape)
+    yield "dispatch", lambda: g.dispatch(make(z(t, d)), r)
+    yield "combine rows", lambda: g.combine(make(z(t * k, d)), r, z(t, k))
+    yield "combine rows alone", lambda: g.combine(make(z(t * k, d)), r)
+    yield "combine weights", lambda: g.combine(z(t * k, d), r, make(z(t, k)))
+    yield "dispatch_backward", lambda: g.dispatch_backward(make(z(t * k, d)), r)
+    yield "combine_backward grad", lambda: g.combine_backward(make(z(t, d)), z(t * k, d), r, z(t, k))
+    yield "combine_backward rows", lambda: g.combine_backward(z(t, d), make(z(t * k, d)), r, z(t, k))
+    yield "combine_backward weights", lambda: g.combine_backward(z(t, d), z(t * k, d), r, make(z(t, k)))
+    args = dict(partials=lambda: z(t, d), residual=lambda: z(t, d), pre_weight=lambda: z(d), post_weight=lambda: z(d), gate=lambda: z(t, 1))
+    for name in args:
+        yield "reduce_norm " + name, lambda name=name: g.reduce_norm(**{n: make(f()) if n == name else f() for n, f in args.items()})
+    yield "reduce_norm one of the partials", lambda: g.reduce_norm([z(t, d), z(t, d), make(z(t, d)), z(t, d)], z(t, d), z(d))
+    saved = block_ops.ReduceNormSaved(1, 4, (t, d), z(t, d), z(2, t), z(t, d), z(d), z(d), z(t, 1), 1.0, 1e-6)
+    yield "reduce_norm_backward hidden", lambda: g.reduce_norm_backward(saved, make(z(t, d)), None)
+    yield "reduce_norm_backward normed", lambda: g.reduce_norm_backward(saved, None, make(z(4, t, d)))
+
+
+def test_tangents_are_refused(recorder):
+    """Forward-mode derivatives: an output without a tangent would be a derivative of zero."""
+    from torch.autograd import forward_ad
+    g, r = recorder, routing()
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for grad in (True, False):                           # no_grad does not switch them off
+            for name, call in every_call(g, r, dual):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+                    pytest.fail(name)
+        with pytest.raises(NotImplementedError):
+            g.dispatch(dual(torch.zeros(3, 8)).requires_grad_(True), r)
+        assert not g.calls
+        for name, call in every_call(g, r):                  # a level alone changes nothing
+            call()
+        with torch.inference_mode():                         # nobody asks for derivatives
+            g.dispatch(dual(torch.zeros(3, 8)), r)
+    assert len(g.calls) == len(list(every_call(g, r))) + 1
