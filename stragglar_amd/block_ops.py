@@ -106,6 +106,26 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+_tracing, _modes, _function_modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._is_torch_function_mode_enabled
+_transforms = torch._C._functorch.peek_interpreter_stack
+
+
+def _refuse_tracers():
+    """The kernels run behind torch's dispatcher: whoever records its operations, or runs them on tensors without
+    memory, gets the allocation of the outputs and nothing that fills them.  A dispatch mode that only watches
+    (counts, logs, decides what to keep) is none of torch's own recorders and stays allowed."""
+    if _modes() or _function_modes() or _tracing() or _transforms() is not None:
+        _refuse_recorders()
+
+
+def _refuse_recorders():
+    inner = _transforms()
+    if (_tracing() or any(m.is_infra_mode() for m in torch.utils._python_dispatch._get_current_dispatch_mode_stack())
+            or torch._C._dispatch_tls_is_dispatch_key_included(torch._C.DispatchKey.PreDispatch)
+            or (inner is not None and inner.key() == torch._C._functorch.TransformType.Functionalize)):
+        raise RuntimeError("the block operators cannot be traced: their kernels are no torch operations")
+
+
 def _refuse_tangents(*tensors):
     """There are no forward-mode derivatives: a tangent would be lost, which reads as a derivative of zero."""
     if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
@@ -141,6 +161,7 @@ class _Node(torch.autograd.Function):
 
     @classmethod
     def _backward(cls, ctx, *grads):
+        _refuse_tracers()
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the backward pass of a call recorded by autograd cannot be captured: capture the *_backward call")
         if torch.is_grad_enabled():
@@ -156,6 +177,7 @@ def _route_workspace(tokens, topk, num_experts):
 
 
 def route(group, experts, num_experts: int) -> Routing:
+    _refuse_tracers()
     if not isinstance(experts, torch.Tensor) or experts.dim() != 2:
         raise ValueError("experts must be a tensor [tokens, topk]")
     tokens, topk = experts.shape
@@ -286,6 +308,7 @@ def _check_weights(routing, weights, dtype):
 
 
 def dispatch(group, tokens, routing):
+    _refuse_tracers()
     if not _fits_rows(group, tokens, routing, False):
         _routing_rows(group, "tokens", tokens, routing, False)
         _on_device(group, tokens=tokens, routing=routing.offsets)
@@ -295,6 +318,7 @@ def dispatch(group, tokens, routing):
 
 
 def combine(group, rows, routing, weights=None):
+    _refuse_tracers()
     if not _fits_rows(group, rows, routing, True):
         _routing_rows(group, "rows", rows, routing, True)
         _check_weights(routing, weights, rows.dtype)
@@ -309,6 +333,7 @@ def combine(group, rows, routing, weights=None):
 
 
 def dispatch_backward(group, grad, routing):
+    _refuse_tracers()
     _routing_rows(group, "grad", grad, routing, True)
     _on_device(group, grad=grad, routing=routing.offsets)
     _refuse_tangents(grad)
@@ -316,6 +341,7 @@ def dispatch_backward(group, grad, routing):
 
 
 def combine_backward(group, grad, rows, routing, weights=None):
+    _refuse_tracers()
     _routing_rows(group, "rows", rows, routing, True)
     _tensor("grad", grad, (routing.tokens, rows.shape[1]), (rows.dtype,))
     _check_weights(routing, weights, rows.dtype)
@@ -492,6 +518,7 @@ def _fits_reduce_norm(group, partials, inputs, residual, pre_weight, post_weight
 
 def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], residual, pre_weight=None, post_weight=None, gate=None,
                 residual_scale: float = 1.0, eps: float = 1e-6, gather: bool = True, save: bool = False):
+    _refuse_tracers()
     inputs = (partials,) if isinstance(partials, torch.Tensor) else tuple(partials)
     addresses = _fits_reduce_norm(group, partials, inputs, residual, pre_weight, post_weight, gate, eps) if inputs else None
     if addresses is None:
@@ -510,6 +537,7 @@ def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], re
 
 
 def reduce_norm_backward(group, saved: ReduceNormSaved, grad_hidden=None, grad_normed=None) -> ReduceNormGrads:
+    _refuse_tracers()
     if not isinstance(saved, ReduceNormSaved):
         raise TypeError("saved must come from reduce_norm(..., save=True)")
     tokens, dim = saved.residual.shape

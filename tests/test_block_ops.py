@@ -295,3 +295,47 @@ def test_tangents_are_refused(recorder):
         with torch.inference_mode():                         # nobody asks for derivatives
             g.dispatch(dual(torch.zeros(3, 8)), r)
     assert len(g.calls) == len(list(every_call(g, r))) + 1
+
+
+def test_tracers_are_refused(recorder):
+    """A recorder of torch's operations would keep the allocation of the outputs and none of the kernels."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    g, r, x = recorder, routing(), torch.zeros(3, 8)
+    ids = torch.zeros(3, 2, dtype=torch.int64)
+    calls = list(every_call(g, r)) + [("route", lambda: g.route(ids, 8))]
+
+    def also(call):
+        def f(t):
+            call()
+            return t + 1
+        return f
+    for name, call in calls:
+        for how in (lambda f: make_fx(f)(x), lambda f: make_fx(f, pre_dispatch=True)(x), lambda f: make_fx(f, tracing_mode="symbolic")(x),
+                    lambda f: torch.jit.trace(f, x, check_trace=False), lambda f: torch.func.functionalize(f)(x)):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                how(also(call))
+                pytest.fail(name)
+        with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(RuntimeError, match="cannot be traced"):
+            call()
+    leaf = x.clone().requires_grad_(True)
+    out = g.dispatch(leaf, r)
+    g.calls.clear()
+    with pytest.raises(RuntimeError, match="cannot be traced"):       # the backward pass of a call made before
+        make_fx(lambda t: torch.autograd.grad(out, leaf, t)[0])(torch.zeros(6, 8))
+    assert not g.calls
+
+
+def test_a_mode_that_watches_changes_nothing(recorder):
+    from torch.utils.flop_counter import FlopCounterMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    g, r = recorder, routing()
+    leaf = torch.zeros(3, 8, requires_grad=True)
+    for mode in (FlopCounterMode(display=False), Log()):
+        with mode:
+            assert torch.autograd.grad(g.dispatch(leaf, r).sum(), leaf)[0].shape == (3, 8)
+    assert g.calls == ["sar_dispatch", "sar_combine"] * 2
