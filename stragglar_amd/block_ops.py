@@ -265,7 +265,9 @@ class _Combine(_Node):
     def forward(ctx, rows, weights, plain):
         group, routing = plain
         ctx.group = group
-        ctx.save_for_backward(rows, weights, _savable(routing.row_of_slot), _savable(routing.offsets))
+        # the rows, tokens * topk of them, are read by the weights' gradient alone
+        kept = rows if weights is not None and ctx.needs_input_grad[1] else None
+        ctx.save_for_backward(kept, weights, _savable(routing.row_of_slot), _savable(routing.offsets))
         return _combine(group, rows, routing.row_of_slot, weights)
 
     @staticmethod

@@ -339,3 +339,21 @@ def test_a_mode_that_watches_changes_nothing(recorder):
         with mode:
             assert torch.autograd.grad(g.dispatch(leaf, r).sum(), leaf)[0].shape == (3, 8)
     assert g.calls == ["sar_dispatch", "sar_combine"] * 2
+
+
+def test_combine_keeps_its_rows_for_the_gradient_of_weights_alone(recorder):
+    g, r = recorder, routing()
+    leaf = torch.zeros(6, 8, requires_grad=True)
+    for weights, kept in [(None, False), (torch.zeros(3, 2), False), (torch.zeros(3, 2, requires_grad=True), True)]:
+        rows = leaf.clone()
+        out = g.combine(rows, r, weights)
+        address = rows.data_ptr()
+        assert (address in [t.data_ptr() for t in out.grad_fn.saved_tensors if t is not None]) == kept
+        rows.add_(1)                                       # in place: only the gradient that reads the rows minds
+        if kept:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(out.sum(), leaf)
+        else:
+            g.calls.clear()
+            assert torch.autograd.grad(out.sum(), leaf)[0].shape == (6, 8)
+            assert g.calls == ["sar_dispatch"]

@@ -826,3 +826,19 @@ def test_a_routing_between_forward_and_backward(groups):
         r.row_of_slot.copy_(again.row_of_slot), r.offsets.copy_(again.offsets)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             outs[0].sum().backward()
+
+
+def test_combine_lets_go_of_rows_that_no_gradient_reads(groups):
+    """Without a gradient of the weights the rows' memory comes back before the backward pass, with the same gradient."""
+    g, t, k, d = groups(4), 4096, 8, 512
+    r = g.route(choices(1, t, k, 8), 8)
+    leaf, w = randn(2, t * k, d).requires_grad_(True), torch.softmax(randn(3, t, k), 1)
+    grad = randn(4, t, d)
+    want = g.combine_backward(grad, leaf.detach(), r, w)[0]
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    rows = leaf * 1.0
+    y = g.combine(rows, r, w)
+    del rows
+    assert torch.cuda.memory_allocated() - before < 2 * t * d * 4           # y, not the 64 MiB of rows
+    assert torch.equal(torch.autograd.grad(y, leaf, grad)[0], want)
