@@ -538,10 +538,33 @@ def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], re
                                            residual_scale, eps)
 
 
+def _check_saved(s: ReduceNormSaved):
+    """Says what is wrong with a saved call: the kernels take its sizes from its residual."""
+    residual = s.residual
+    if not isinstance(residual, torch.Tensor) or residual.dim() != 2:
+        raise ValueError("saved.residual must be a tensor [tokens, dim]")
+    _tensor("saved.residual", residual, dtypes=DTYPE_CODES)
+    (tokens, dim), dtype = residual.shape, residual.dtype
+    kinds = (torch.float32, dtype)
+    _tensor("saved.total", s.total, (tokens, dim), kinds)
+    _tensor("saved.stats", s.stats, (2, tokens), (torch.float32,))
+    if tuple(s.partial_shape) not in ((s.sources, tokens, dim), (tokens, dim)[:2 if s.sources == 1 else 0]):
+        raise ValueError("saved.partial_shape is %s with %d sources of %s" % (tuple(s.partial_shape), s.sources, (tokens, dim)))
+    if s.pre_weight is not None:
+        _tensor("saved.pre_weight", s.pre_weight, (dim,), kinds)
+    if s.post_weight is not None:
+        _tensor("saved.post_weight", s.post_weight, (dim,), kinds)
+    if s.gate is not None:
+        _tensor("saved.gate", s.gate, dtypes=kinds)
+        if tuple(s.gate.shape) not in ((dim,), (tokens, 1), (tokens, dim)):
+            raise ValueError("saved.gate must be [dim], [tokens, 1] or [tokens, dim]: got %s" % (tuple(s.gate.shape),))
+
+
 def reduce_norm_backward(group, saved: ReduceNormSaved, grad_hidden=None, grad_normed=None) -> ReduceNormGrads:
     _refuse_tracers()
     if not isinstance(saved, ReduceNormSaved):
         raise TypeError("saved must come from reduce_norm(..., save=True)")
+    _check_saved(saved)
     tokens, dim = saved.residual.shape
     if grad_hidden is not None:
         _tensor("grad_hidden", grad_hidden, (tokens, dim), (saved.residual.dtype,))
@@ -552,6 +575,7 @@ def reduce_norm_backward(group, saved: ReduceNormSaved, grad_hidden=None, grad_n
         if tuple(grad_normed.shape) not in ok:
             raise ValueError("grad_normed has shape %s, need %s" % (tuple(grad_normed.shape), ok[-1]))
         _tensor("grad_normed", grad_normed, dtypes=(saved.residual.dtype,))
-    _on_device(group, grad_hidden=grad_hidden, grad_normed=grad_normed, residual=saved.residual)
+    _on_device(group, grad_hidden=grad_hidden, grad_normed=grad_normed, residual=saved.residual, total=saved.total, stats=saved.stats,
+               pre_weight=saved.pre_weight, post_weight=saved.post_weight, gate=saved.gate)
     _refuse_tangents(grad_hidden, grad_normed, saved.total, saved.residual, saved.pre_weight, saved.post_weight, saved.gate)
     return _reduce_norm_backward(group, saved, grad_hidden, grad_normed, (True,) * 5)

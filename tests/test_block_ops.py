@@ -357,3 +357,26 @@ def test_combine_keeps_its_rows_for_the_gradient_of_weights_alone(recorder):
             g.calls.clear()
             assert torch.autograd.grad(out.sum(), leaf)[0].shape == (6, 8)
             assert g.calls == ["sar_dispatch"]
+
+
+def test_a_saved_call_is_checked_part_by_part(recorder):
+    """The kernels take a saved call's sizes from its residual: parts that do not fit it would be read past their ends."""
+    g, t, d = recorder, 3, 8
+    z = torch.zeros
+    saved = block_ops.ReduceNormSaved(4, 4, (4, t, d), z(t, d), z(2, t), z(t, d).half(), z(d), z(d).half(), z(t, 1), 1.0, 1e-6)
+    grad = z(t, d).half()
+    assert g.reduce_norm_backward(saved, grad).partials.shape == (4, t, d) and g.calls == ["sar_reduce_norm_backward"]
+    one = saved._replace(sources=1, partial_shape=(t, d), total=z(t, d).half())
+    assert g.reduce_norm_backward(one, grad).partials.shape == (t, d)
+    g.calls.clear()
+    for part in [dict(total=z(t - 1, d)), dict(total=z(t, d).double()), dict(total=z(d, t).t()), dict(total=None), dict(stats=z(2, t - 1)), dict(stats=z(2, t).half()),
+                 dict(stats=z(t, 2).t()), dict(residual=z(t * d).half()), dict(residual=None), dict(residual=z(t + 1, d).half()), dict(partial_shape=(3, t, d)),
+                 dict(partial_shape=(t, d)), dict(partial_shape=()), dict(sources=5), dict(pre_weight=z(d - 1)), dict(pre_weight=z(d).double()),
+                 dict(post_weight=z(2 * d)[::2]), dict(gate=z(t)), dict(gate=z(t, 1).double()), dict(gate=z(1, d))]:
+        with pytest.raises((ValueError, TypeError), match=list(part)[0] if "residual" not in part and "sources" not in part else "saved"):
+            g.reduce_norm_backward(saved._replace(**part), grad)
+            pytest.fail(str(part))
+    g.device = 0
+    with pytest.raises(ValueError, match="CUDA"):
+        g.reduce_norm_backward(saved)
+    assert not g.calls
