@@ -548,8 +548,9 @@ def _check_saved(s: ReduceNormSaved):
     kinds = (torch.float32, dtype)
     _tensor("saved.total", s.total, (tokens, dim), kinds)
     _tensor("saved.stats", s.stats, (2, tokens), (torch.float32,))
-    if tuple(s.partial_shape) not in ((s.sources, tokens, dim), (tokens, dim)[:2 if s.sources == 1 else 0]):
-        raise ValueError("saved.partial_shape is %s with %d sources of %s" % (tuple(s.partial_shape), s.sources, (tokens, dim)))
+    shape = tuple(s.partial_shape)
+    if shape != (s.sources, tokens, dim) and not (s.sources == 1 and shape == (tokens, dim)):
+        raise ValueError("saved.partial_shape is %s with %s sources of %s" % (shape, s.sources, (tokens, dim)))
     if s.pre_weight is not None:
         _tensor("saved.pre_weight", s.pre_weight, (dim,), kinds)
     if s.post_weight is not None:
