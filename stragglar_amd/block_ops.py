@@ -243,17 +243,26 @@ def _savable(t):
     return t.clone() if t.is_inference() else t
 
 
+def _given_back(group, t, dtype, shape):
+    """A saved tensor as autograd gives it back.  Saved-tensor hooks come in between: what they return in another type,
+    size, order or place would be read as what it was."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != group.device or not t.is_contiguous():
+        raise RuntimeError("a saved-tensor hook gave back %s %s on %s instead of a contiguous %s %s on device %d"
+                           % (t.dtype, tuple(t.shape), t.device, dtype, tuple(shape), group.device))
+    return t
+
+
 class _Dispatch(_Node):
     @staticmethod
     def forward(ctx, rows, plain):
-        group, routing = plain
-        ctx.group = group
+        ctx.group, routing = plain
+        ctx.size = routing.row_of_slot.shape
         ctx.save_for_backward(_savable(routing.row_of_slot))
-        return _dispatch(group, rows, routing.row_of_slot, routing.offsets)
+        return _dispatch(ctx.group, rows, routing.row_of_slot, routing.offsets)
 
     @staticmethod
     def gradients(ctx, grad):
-        return _combine(ctx.group, grad.contiguous(), ctx.saved_tensors[0]), None
+        return _combine(ctx.group, grad.contiguous(), _given_back(ctx.group, ctx.saved_tensors[0], torch.int32, ctx.size)), None
 
     @staticmethod
     def backward(ctx, grad):
@@ -263,18 +272,24 @@ class _Dispatch(_Node):
 class _Combine(_Node):
     @staticmethod
     def forward(ctx, rows, weights, plain):
-        group, routing = plain
-        ctx.group = group
+        ctx.group, routing = plain
+        ctx.size, ctx.offsets = routing.row_of_slot.shape, routing.offsets.shape
+        ctx.weights = weights.dtype if weights is not None else None
         # the rows, tokens * topk of them, are read by the weights' gradient alone
         kept = rows if weights is not None and ctx.needs_input_grad[1] else None
         ctx.save_for_backward(kept, weights, _savable(routing.row_of_slot), _savable(routing.offsets))
-        return _combine(group, rows, routing.row_of_slot, weights)
+        return _combine(ctx.group, rows, routing.row_of_slot, weights)
 
     @staticmethod
     def gradients(ctx, grad):
         rows, weights, row_of_slot, offsets = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        a, b = _combine_backward(ctx.group, grad.contiguous(), rows, row_of_slot, offsets, weights, need[0], weights is not None and need[1])
+        group, size, need = ctx.group, ctx.size, ctx.needs_input_grad
+        _given_back(group, row_of_slot, torch.int32, size), _given_back(group, offsets, torch.int32, ctx.offsets)
+        if rows is not None:
+            _given_back(group, rows, grad.dtype, (size[0] * size[1], grad.shape[1]))
+        if weights is not None:
+            _given_back(group, weights, ctx.weights, size)
+        a, b = _combine_backward(group, grad.contiguous(), rows, row_of_slot, offsets, weights, need[0], weights is not None and need[1])
         return a, b, None
 
     @staticmethod
@@ -431,14 +446,20 @@ class _ReduceNorm(_Node):
         hidden, normed, total, stats = _reduce_norm(group, partials[0], addresses, residual, pre_weight, post_weight, gate, residual_scale, eps,
                                                     gather, True)
         ctx.plain = plain
-        ctx.save_for_backward(total, stats, residual, pre_weight, post_weight, gate)
+        kept = (total, stats, residual, pre_weight, post_weight, gate)
+        ctx.kept = [(t.dtype, t.shape) if t is not None else None for t in kept]
+        ctx.save_for_backward(*kept)
         ctx.set_materialize_grads(False)
         return hidden, normed
 
     @staticmethod
     def gradients(ctx, grad_hidden, grad_normed):
-        total, stats, residual, pre_weight, post_weight, gate = ctx.saved_tensors
         group, shape, addresses, residual_scale, eps, gather = ctx.plain
+        kept = ctx.saved_tensors
+        for t, was in zip(kept, ctx.kept):
+            if was is not None:
+                _given_back(group, t, *was)
+        total, stats, residual, pre_weight, post_weight, gate = kept
         saved = ReduceNormSaved(len(addresses), group.n if gather else 1, shape, total, stats, residual, pre_weight,
                                 post_weight, gate, residual_scale, eps)
         need = ctx.needs_input_grad

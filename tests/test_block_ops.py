@@ -380,3 +380,37 @@ def test_a_saved_call_is_checked_part_by_part(recorder):
     with pytest.raises(ValueError, match="CUDA"):
         g.reduce_norm_backward(saved)
     assert not g.calls
+
+
+def test_what_saved_tensor_hooks_give_back_is_checked(recorder):
+    """Hooks may move saved tensors away and bring them back; what comes back in another type, size or order is refused
+    before a kernel reads it as what it was."""
+    g, r, z = recorder, routing(), torch.zeros
+    x, rows, w = z(3, 8, requires_grad=True), z(6, 8, requires_grad=True), z(3, 2, requires_grad=True)
+    d = z(8, requires_grad=True)
+    calls = [("sar_combine", lambda: g.dispatch(x, r), x), ("sar_dispatch", lambda: g.combine(rows, r), rows), ("sar_dispatch", lambda: g.combine(rows, r, w.detach()), rows),
+             ("sar_combine_backward", lambda: g.combine(rows, r, w), w), ("sar_reduce_norm_backward", lambda: g.reduce_norm([x] * 4, x, d, d, d)[0], d)]
+    bad = [lambda t: t.to(torch.float16), lambda t: t[:-1], lambda t: t.unsqueeze(0), lambda t: torch.stack([t, t], -1)[..., 0]]
+    for entry, call, leaf in calls:
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.numpy(force=True).copy(), torch.from_numpy):
+            out = call()
+            g.calls.clear()
+            torch.autograd.grad(out.sum(), leaf)
+        assert g.calls == [entry]
+        for change in bad:
+            at = 0                                       # each saved tensor in turn
+            while True:
+                seen = []
+
+                def unpack(t):
+                    seen.append(t)
+                    return change(t) if len(seen) == at + 1 else t
+                with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), unpack):
+                    out = call()
+                if at == sum(t is not None for t in out.grad_fn.saved_tensors):
+                    break
+                g.calls.clear(), seen.clear()
+                with pytest.raises(RuntimeError, match="saved-tensor hook"):
+                    torch.autograd.grad(out.sum(), leaf)
+                assert not g.calls, (entry, at)
+                at += 1

@@ -842,3 +842,23 @@ def test_combine_lets_go_of_rows_that_no_gradient_reads(groups):
     del rows
     assert torch.cuda.memory_allocated() - before < 2 * t * d * 4           # y, not the 64 MiB of rows
     assert torch.equal(torch.autograd.grad(y, leaf, grad)[0], want)
+
+
+def test_saved_tensors_kept_on_the_host(groups):
+    """Offloaded and brought back they give the same bits; left on the host they are refused before a kernel sees them."""
+    g, t, k, d = groups(4), 60, 2, 72
+    r = g.route(choices(1, t, k, 8, 0.2), 8)
+    x, w, v = randn(2, t, d).requires_grad_(True), torch.softmax(randn(3, t, k), 1).requires_grad_(True), randn(4, d, mean=1.0, scale=0.1).requires_grad_(True)
+
+    def forward():
+        y = g.combine(g.dispatch(x, r), r, w)
+        return g.reduce_norm([y, x, y, x], x, pre_weight=v, post_weight=v, gate=v)[1]
+    want = torch.autograd.grad(forward().square().sum(), (x, w, v))
+    with torch.autograd.graph.save_on_cpu():
+        out = forward()
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out.square().sum(), (x, w, v)), want))
+    for call in (lambda: g.dispatch(x, r), lambda: g.combine(x[:1].expand(t * k, -1).contiguous(), r, w), lambda: g.reduce_norm(x, x, v)[1]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s.cpu(), lambda s: s):
+            out = call()
+        with pytest.raises(RuntimeError, match="saved-tensor hook"):
+            out.backward(torch.ones_like(out))
