@@ -542,6 +542,8 @@ def _fits_reduce_norm(group, partials, inputs, residual, pre_weight, post_weight
 def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], residual, pre_weight=None, post_weight=None, gate=None,
                 residual_scale: float = 1.0, eps: float = 1e-6, gather: bool = True, save: bool = False):
     _refuse_tracers()
+    if isinstance(residual_scale, torch.Tensor) or isinstance(eps, torch.Tensor):
+        raise TypeError("residual_scale and eps are numbers: a tensor's value would be waited for, and get no gradient")
     inputs = (partials,) if isinstance(partials, torch.Tensor) else tuple(partials)
     addresses = _fits_reduce_norm(group, partials, inputs, residual, pre_weight, post_weight, gate, eps) if inputs else None
     if addresses is None:

@@ -414,3 +414,16 @@ def test_what_saved_tensor_hooks_give_back_is_checked(recorder):
                     torch.autograd.grad(out.sum(), leaf)
                 assert not g.calls, (entry, at)
                 at += 1
+
+
+def test_scale_and_eps_are_numbers(recorder):
+    """A tensor would be turned into a number behind autograd's back, its gradient lost."""
+    x, learned = torch.zeros(3, 8), torch.tensor(0.5, requires_grad=True)
+    for bad in (learned, learned.detach()):
+        with pytest.raises(TypeError, match="numbers"):
+            recorder.reduce_norm(x, x, residual_scale=bad)
+        with pytest.raises(TypeError, match="numbers"):
+            recorder.reduce_norm(x, x, eps=bad)
+    assert not recorder.calls
+    for scale, eps in ((1, 0), (0.5, 1e-6), (-0.25, 1e-5)):
+        recorder.reduce_norm(x, x, residual_scale=scale, eps=eps)
