@@ -134,6 +134,14 @@ def _refuse_tangents(*tensors):
                 raise NotImplementedError("the block operators have no forward-mode derivatives")
 
 
+def _capturing(device: int) -> bool:
+    """Whether the current stream of `device`, which need not be the current device, is being captured."""
+    if device < 0 or device == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _recording(*tensors) -> bool:
     """Whether autograd has to record the call."""
     if forward_ad._current_level >= 0:
@@ -145,7 +153,7 @@ def _recording(*tensors) -> bool:
             break
     else:
         return False
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing(t.get_device()):
         raise RuntimeError("gradients cannot be recorded while a stream is being captured: call this under torch.no_grad() "
                            "and the *_backward call in the same capture")
     return True

@@ -427,3 +427,32 @@ def test_scale_and_eps_are_numbers(recorder):
     assert not recorder.calls
     for scale, eps in ((1, 0), (0.5, 1e-6), (-0.25, 1e-5)):
         recorder.reduce_norm(x, x, residual_scale=scale, eps=eps)
+
+
+def test_the_capture_check_asks_the_tensors_own_device(monkeypatch):
+    """With another device current it is the stream of the tensors' device that counts, in either direction."""
+    import contextlib
+    now = [0]
+
+    @contextlib.contextmanager
+    def device(d):
+        before, now[0] = now[0], d
+        yield
+        now[0] = before
+
+    class Leaf:
+        requires_grad = True
+
+        def __init__(self, device):
+            self.device_index = device
+
+        def get_device(self):
+            return self.device_index
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] == 1)
+    with pytest.raises(RuntimeError, match="captured"):
+        block_ops._recording(None, Leaf(1))
+    assert block_ops._recording(Leaf(0)) and now == [0]
+    now[0] = 1
+    assert block_ops._recording(Leaf(0)) and now == [1]
