@@ -862,3 +862,86 @@ def test_saved_tensors_kept_on_the_host(groups):
             out = call()
         with pytest.raises(RuntimeError, match="saved-tensor hook"):
             out.backward(torch.ones_like(out))
+
+
+# ---- every kernel's streaming form (calls of 512 MiB and more) -----------------------------------------------------
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 512), ("f16", 505), ("f32", 520), ("bf16", 1001), ("f16", 2041), ("f32", 1024)])
+def test_streaming_gradients_of_short_rows(groups, dtype, dim):
+    """combine's gradients where a wave has a token to itself: rows of up to 64, 128 and 256 vectors.  With and without a
+    gradient of the weights (then the rows' is a weighted dispatch)."""
+    g, dt, topk = groups(8), DT[dtype], 8
+    row = dim * torch.finfo(dt).bits // 8
+    t = (530 << 20) // (topk * row)                                # rows alone pass 512 MiB
+    assert t >= 2048 and row <= 256 * 16
+    r = g.route(choices(dim, t, topk, 16, 0.05), 16)
+    index, has, total = r.row_of_slot.long(), r.row_of_slot >= 0, int(r.offsets[-1])
+    base = randn(1, 499, dim, dtype=dt)
+    rows = base[torch.arange(t * topk, device="cuda") % 499].requires_grad_(True)
+    grad = base[torch.arange(t, device="cuda") * 5 % 499]
+    w = randn(2, t, topk, scale=0.5)
+    alone, = torch.autograd.grad(g.combine(rows, r, w), rows, grad)
+    gr, gw = g.combine_backward(grad, rows.detach(), r, w)
+    assert torch.equal(alone, gr)
+    assert not gr[total:].any() and not gw[~has].any()
+    y = g.combine(rows.detach(), r, w)
+    for a in (0, t // 3, t - 40):
+        part = slice(a, a + 40)
+        i, h = index[part], has[part]
+        taken = torch.where(h.unsqueeze(2), rows.detach()[i.clamp(min=0)].double(), torch.zeros((), dtype=torch.float64, device="cuda"))
+        check(y[part], (B(taken) * B(w[part].unsqueeze(2))).sum(1, topk), a)
+        check(gw[part], (B(grad[part].unsqueeze(1).expand_as(taken)) * B(taken)).sum(2, dim // 64 + 64), a)
+        check(gr[i[h]], B(grad[part].unsqueeze(1).expand(-1, topk, -1)[h]) * B(w[part][h].unsqueeze(1)), a)
+
+
+@pytest.mark.parametrize("dtype,dim,n,partials,gather,gate", [
+    ("bf16", 9001, 3, "ranks", True, "channel"), ("f16", 16384, 4, "ranks", False, "full"), ("f32", 5000, 3, "ranks", True, "token"),
+    ("f32", 16384, 3, "ranks", True, "channel"), ("f32", 8193, 3, "one", False, "channel"), ("bf16", 16383, 3, "one", False, "channel"),
+    ("bf16", 256, 4, "ranks", True, "channel"), ("f16", 250, 4, "one", False, "channel"), ("f32", 516, 8, "ranks", True, "none"), ("bf16", 4096, 3, "one", False, "token")])
+def test_streaming_norms(groups, dtype, dim, n, partials, gather, gate):
+    """Rows of two and four vectors a thread (their column sums in LDS), rows that share a workgroup, and finished outputs.
+    Column sums add at most tokens / (workgroups * rows) + rows + workgroups / 32 + 32 times in a row: 122 for rows of 250, 82
+    and less for the others, so 1.25 times what COLUMN allows holds for all."""
+    g, dt, scale, eps = groups(n), DT[dtype], 0.75, 1e-6
+    sources, copies = n if partials == "ranks" else 1, n if gather else 1
+    row = dim * torch.finfo(dt).bits // 8
+    t = (513 << 20) // ((sources + copies + 2) * row) + 1           # the rows that the smallest pass counts
+    spread = torch.arange(t, device="cuda")
+    base = [randn(r, 499, dim, dtype=dt) for r in range(4)]
+    parts = [base[r % 4][(spread * (r + 1) + r) % 499] * n ** -0.5 for r in range(sources)]
+    shape = {"none": None, "channel": (dim,), "token": (t, 1), "full": (t, dim)}[gate]
+    s = dict(partials=parts if partials == "ranks" else parts[0], residual=base[3][(spread * 3) % 499],
+             pre_weight=randn(5, dim, mean=1.0, scale=0.2), post_weight=randn(6, dim, mean=1.0, scale=0.2),
+             gate=None if shape is None else randn(7, *shape, mean=0.5, scale=0.2))
+    gh = base[0][(spread * 7) % 499]
+    gx = torch.stack([base[r % 4][(spread * 11 + r) % 499] for r in range(copies)])
+    with torch.no_grad():
+        hidden, normed, saved = run_norm(g, s, scale, eps, gather, save=True)
+        back = g.reduce_norm_backward(saved, gh, gx if gather else gx[0])
+        again = run_norm(g, s, scale, eps, gather)                                  # without a total to write
+    assert torch.equal(again[0], hidden) and torch.equal(again[1], normed)
+    del again
+
+    def cut(part):
+        p = [q[part] for q in s["partials"]] if partials == "ranks" else s["partials"][part]
+        q = dict(s, partials=p, residual=s["residual"][part])
+        if gate in ("token", "full"):
+            q["gate"] = s["gate"][part]
+        return plain_norm(q, scale, eps, gh[part], gx[:, part])
+    sums = {}
+    for a in range(0, t, 2000):
+        part = slice(a, min(t, a + 2000))
+        h, x, want = cut(part)
+        for k in ("pre_weight", "post_weight") + (("gate",) if gate == "channel" else ()):
+            v, e = sums.get(k, (0, 0))
+            sums[k] = (v + want[k].v, e + want[k].e)
+        if a in (0, t // 4000 * 2000) or part.stop == t:
+            check(hidden[part], h, a), check(back.residual[part], want["residual"], a)
+            for q in (normed if gather else [normed]):
+                check(q[part], x, a)
+            for q in (back.partials if partials == "ranks" else [back.partials]):
+                check(q[part], want["partials"], a)
+            if gate in ("token", "full"):
+                check(back.gate[part], want["gate"], a)
+    for k, (v, e) in sums.items():
+        check(getattr(back, k), B(v, 1.25 * e), k)
