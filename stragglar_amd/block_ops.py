@@ -251,26 +251,31 @@ def _savable(t):
     return t.clone() if t.is_inference() else t
 
 
+_HOOKED = "a saved-tensor hook gave back a tensor of another type, size, order or device than it was given"
+_hooks = torch._C._autograd._top_saved_tensors_default_hooks      # those in force, or None: asked when tensors are saved
+
+
 def _given_back(group, t, dtype, shape):
     """A saved tensor as autograd gives it back.  Saved-tensor hooks come in between: what they return in another type,
     size, order or place would be read as what it was."""
     if t.dtype is not dtype or t.shape != shape or t.get_device() != group.device or not t.is_contiguous():
-        raise RuntimeError("a saved-tensor hook gave back %s %s on %s instead of a contiguous %s %s on device %d"
-                           % (t.dtype, tuple(t.shape), t.device, dtype, tuple(shape), group.device))
-    return t
+        raise RuntimeError(_HOOKED)
 
 
 class _Dispatch(_Node):
     @staticmethod
     def forward(ctx, rows, plain):
-        ctx.group, routing = plain
-        ctx.size = routing.row_of_slot.shape
+        group, routing = plain
+        ctx.plain = (group, routing.row_of_slot.shape, _hooks(True))
         ctx.save_for_backward(_savable(routing.row_of_slot))
-        return _dispatch(ctx.group, rows, routing.row_of_slot, routing.offsets)
+        return _dispatch(group, rows, routing.row_of_slot, routing.offsets)
 
     @staticmethod
     def gradients(ctx, grad):
-        return _combine(ctx.group, grad.contiguous(), _given_back(ctx.group, ctx.saved_tensors[0], torch.int32, ctx.size)), None
+        (group, size, hooked), (row_of_slot,) = ctx.plain, ctx.saved_tensors
+        if hooked:
+            _given_back(group, row_of_slot, torch.int32, size)
+        return _combine(group, grad.contiguous(), row_of_slot), None
 
     @staticmethod
     def backward(ctx, grad):
@@ -280,23 +285,26 @@ class _Dispatch(_Node):
 class _Combine(_Node):
     @staticmethod
     def forward(ctx, rows, weights, plain):
-        ctx.group, routing = plain
-        ctx.size, ctx.offsets = routing.row_of_slot.shape, routing.offsets.shape
-        ctx.weights = weights.dtype if weights is not None else None
+        group, routing = plain
+        hooked = _hooks(True) and (routing.row_of_slot.shape, routing.offsets.shape, weights.dtype if weights is not None else None)
+        ctx.plain = (group, hooked)
         # the rows, tokens * topk of them, are read by the weights' gradient alone
         kept = rows if weights is not None and ctx.needs_input_grad[1] else None
         ctx.save_for_backward(kept, weights, _savable(routing.row_of_slot), _savable(routing.offsets))
-        return _combine(ctx.group, rows, routing.row_of_slot, weights)
+        return _combine(group, rows, routing.row_of_slot, weights)
 
     @staticmethod
     def gradients(ctx, grad):
         rows, weights, row_of_slot, offsets = ctx.saved_tensors
-        group, size, need = ctx.group, ctx.size, ctx.needs_input_grad
-        _given_back(group, row_of_slot, torch.int32, size), _given_back(group, offsets, torch.int32, ctx.offsets)
-        if rows is not None:
-            _given_back(group, rows, grad.dtype, (size[0] * size[1], grad.shape[1]))
-        if weights is not None:
-            _given_back(group, weights, ctx.weights, size)
+        (group, hooked), need = ctx.plain, ctx.needs_input_grad
+        if hooked:
+            size, ends, weight_dtype = hooked
+            _given_back(group, row_of_slot, torch.int32, size)
+            _given_back(group, offsets, torch.int32, ends)
+            if rows is not None:
+                _given_back(group, rows, grad.dtype, (size[0] * size[1], grad.shape[1]))
+            if weights is not None:
+                _given_back(group, weights, weight_dtype, size)
         a, b = _combine_backward(group, grad.contiguous(), rows, row_of_slot, offsets, weights, need[0], weights is not None and need[1])
         return a, b, None
 
@@ -320,11 +328,14 @@ def _routing_rows(group, name, t, routing, sorted_rows):
 
 def _fits_rows(group, t, routing, sorted_rows):
     """Whether the checks above and of the device pass, in as little time as they take."""
-    if not isinstance(t, torch.Tensor) or not isinstance(routing, Routing) or t.dim() != 2:
+    if not isinstance(t, torch.Tensor) or not isinstance(routing, Routing):
+        return False
+    size = t.shape
+    if len(size) != 2:
         return False
     tokens, topk = routing.row_of_slot.shape
-    return (t.shape[0] == (tokens * topk if sorted_rows else tokens) and t.dtype in DTYPE_CODES and t.is_contiguous()
-            and t.get_device() == group.device and routing.offsets.get_device() == group.device and 1 <= t.shape[1] <= 1 << 24)
+    return (size[0] == (tokens * topk if sorted_rows else tokens) and t.dtype in DTYPE_CODES and t.is_contiguous()
+            and t.get_device() == group.device and routing.offsets.get_device() == group.device and 1 <= size[1] <= 1 << 24)
 
 
 def _check_weights(routing, weights, dtype):
@@ -359,8 +370,9 @@ def combine(group, rows, routing, weights=None):
 
 def dispatch_backward(group, grad, routing):
     _refuse_tracers()
-    _routing_rows(group, "grad", grad, routing, True)
-    _on_device(group, grad=grad, routing=routing.offsets)
+    if not _fits_rows(group, grad, routing, True):
+        _routing_rows(group, "grad", grad, routing, True)
+        _on_device(group, grad=grad, routing=routing.offsets)
     _refuse_tangents(grad)
     return _combine(group, grad, routing.row_of_slot)
 
@@ -453,23 +465,19 @@ class _ReduceNorm(_Node):
         group, shape, addresses, residual_scale, eps, gather = plain
         hidden, normed, total, stats = _reduce_norm(group, partials[0], addresses, residual, pre_weight, post_weight, gate, residual_scale, eps,
                                                     gather, True)
-        ctx.plain = plain
-        kept = (total, stats, residual, pre_weight, post_weight, gate)
-        ctx.kept = [(t.dtype, t.shape) if t is not None else None for t in kept]
-        ctx.save_for_backward(*kept)
+        ctx.plain, ctx.hooked = plain, _hooks(True) and residual.dtype
+        ctx.save_for_backward(total, stats, residual, pre_weight, post_weight, gate)
         ctx.set_materialize_grads(False)
         return hidden, normed
 
     @staticmethod
     def gradients(ctx, grad_hidden, grad_normed):
         group, shape, addresses, residual_scale, eps, gather = ctx.plain
-        kept = ctx.saved_tensors
-        for t, was in zip(kept, ctx.kept):
-            if was is not None:
-                _given_back(group, t, *was)
-        total, stats, residual, pre_weight, post_weight, gate = kept
+        total, stats, residual, pre_weight, post_weight, gate = ctx.saved_tensors
         saved = ReduceNormSaved(len(addresses), group.n if gather else 1, shape, total, stats, residual, pre_weight,
                                 post_weight, gate, residual_scale, eps)
+        if ctx.hooked and (residual.dtype is not ctx.hooked or residual.shape != shape[-2:] or not _fits_saved(group, saved)):
+            raise RuntimeError(_HOOKED)
         need = ctx.needs_input_grad
         g = _reduce_norm_backward(group, saved, grad_hidden.contiguous() if grad_hidden is not None else None,
                                   grad_normed.contiguous() if grad_normed is not None else None, (True in need[5:], need[1], need[2], need[3], need[4]))
@@ -569,6 +577,28 @@ def reduce_norm(group, partials: Union[torch.Tensor, Sequence[torch.Tensor]], re
                                            residual_scale, eps)
 
 
+def _fits_parameter(t, kinds, dim, device):
+    return t is None or (isinstance(t, torch.Tensor) and t.dtype in kinds and t.shape == (dim,) and t.get_device() == device and t.is_contiguous())
+
+
+def _fits_saved(group, s: ReduceNormSaved):
+    """The checks below and of the devices in as little time as they take."""
+    residual, total, stats, gate = s.residual, s.total, s.stats, s.gate
+    if not isinstance(residual, torch.Tensor) or not isinstance(total, torch.Tensor) or not isinstance(stats, torch.Tensor):
+        return False
+    size, dtype, device = residual.shape, residual.dtype, group.device
+    if len(size) != 2 or dtype not in DTYPE_CODES:
+        return False
+    tokens, dim = size
+    kinds, shape = (torch.float32, dtype), tuple(s.partial_shape)
+    return ((shape == (s.sources, tokens, dim) or (s.sources == 1 and shape == size)) and residual.get_device() == device and residual.is_contiguous()
+            and total.shape == size and total.dtype in kinds and total.get_device() == device and total.is_contiguous()
+            and stats.shape == (2, tokens) and stats.dtype is torch.float32 and stats.get_device() == device and stats.is_contiguous()
+            and _fits_parameter(s.pre_weight, kinds, dim, device) and _fits_parameter(s.post_weight, kinds, dim, device)
+            and (gate is None or (isinstance(gate, torch.Tensor) and gate.dtype in kinds and tuple(gate.shape) in ((dim,), (tokens, 1), (tokens, dim))
+                                  and gate.get_device() == device and gate.is_contiguous())))
+
+
 def _check_saved(s: ReduceNormSaved):
     """Says what is wrong with a saved call: the kernels take its sizes from its residual."""
     residual = s.residual
@@ -592,10 +622,19 @@ def _check_saved(s: ReduceNormSaved):
             raise ValueError("saved.gate must be [dim], [tokens, 1] or [tokens, dim]: got %s" % (tuple(s.gate.shape),))
 
 
-def reduce_norm_backward(group, saved: ReduceNormSaved, grad_hidden=None, grad_normed=None) -> ReduceNormGrads:
-    _refuse_tracers()
-    if not isinstance(saved, ReduceNormSaved):
-        raise TypeError("saved must come from reduce_norm(..., save=True)")
+def _fits_grads(group, s: ReduceNormSaved, grad_hidden, grad_normed):
+    """The checks below of the gradients."""
+    size, dtype, device = s.residual.shape, s.residual.dtype, group.device
+    if grad_hidden is not None and not (isinstance(grad_hidden, torch.Tensor) and grad_hidden.shape == size and grad_hidden.dtype is dtype
+                                        and grad_hidden.get_device() == device and grad_hidden.is_contiguous()):
+        return False
+    return grad_normed is None or (
+        s.pre_weight is not None and isinstance(grad_normed, torch.Tensor) and grad_normed.dtype is dtype and grad_normed.get_device() == device
+        and grad_normed.is_contiguous() and (grad_normed.shape == (s.copies, *size) or (s.copies == 1 and grad_normed.shape == size)))
+
+
+def _check_reduce_norm_backward(group, saved, grad_hidden, grad_normed):
+    """Says what is wrong with the arguments of reduce_norm_backward."""
     _check_saved(saved)
     tokens, dim = saved.residual.shape
     if grad_hidden is not None:
@@ -609,5 +648,14 @@ def reduce_norm_backward(group, saved: ReduceNormSaved, grad_hidden=None, grad_n
         _tensor("grad_normed", grad_normed, dtypes=(saved.residual.dtype,))
     _on_device(group, grad_hidden=grad_hidden, grad_normed=grad_normed, residual=saved.residual, total=saved.total, stats=saved.stats,
                pre_weight=saved.pre_weight, post_weight=saved.post_weight, gate=saved.gate)
+    raise ValueError("the arguments do not fit each other")
+
+
+def reduce_norm_backward(group, saved: ReduceNormSaved, grad_hidden=None, grad_normed=None) -> ReduceNormGrads:
+    _refuse_tracers()
+    if not isinstance(saved, ReduceNormSaved):
+        raise TypeError("saved must come from reduce_norm(..., save=True)")
+    if not _fits_saved(group, saved) or not _fits_grads(group, saved, grad_hidden, grad_normed):
+        _check_reduce_norm_backward(group, saved, grad_hidden, grad_normed)
     _refuse_tangents(grad_hidden, grad_normed, saved.total, saved.residual, saved.pre_weight, saved.post_weight, saved.gate)
     return _reduce_norm_backward(group, saved, grad_hidden, grad_normed, (True,) * 5)
