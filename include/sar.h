@@ -567,7 +567,8 @@ typedef struct sar_reduce_norm_grads {
     void* grad_pre_weight;    /* dim, in pre_dtype                                                                  */
     void* grad_post_weight;   /* dim, in post_dtype                                                                 */
     void* grad_gate;          /* as gate, in gate_dtype                                                             */
-    void* workspace;          /* sar_reduce_norm_workspace() bytes (0 for few tokens: may be NULL)                  */
+    void* workspace;          /* sar_reduce_norm_workspace() bytes, whichever gradients are wanted (0 for few tokens:
+                                 may be NULL)                                                                        */
     uint64_t workspace_bytes;
 } sar_reduce_norm_grads;
 uint64_t sar_reduce_norm_workspace(int64_t tokens, int64_t dim, int dtype);

@@ -571,9 +571,11 @@ __global__ __launch_bounds__(kMoveThreads) void combine_backward_kernel(const Mo
 
 // ---- sum over the ranks, norms, gate, residual ----------------------------------------------------------------
 // A workgroup takes one token; its row stays in registers in 32 bits from the sum over the ranks to the last norm, one
-// 16-byte vector a thread as long as 1024 threads reach (two at 4096 columns: 228 us against 220 for eight ranks' 8192
-// tokens, 6.3 against 5.4 for eight tokens).  Bound by HBM: those 8192 tokens of 4096 in bf16 with a copy of the result for
-// every rank (1.2 GB) 205 us, 5.9 TB/s.  A grid that stays and keeps its weights in registers was slower (240).
+// 16-byte vector a thread as long as 1024 threads reach.  Two vectors, from eight ranks in bf16: 6.4 us against 5.1 for 16
+// tokens of 4096, 15.8 against 14.3 for 1024 of 2048, level to 5 % slower from 302 MB on, but 16 to 18 % faster in the three
+// calls measured that move 151 MB (1024 of 4096: 27.2 against 32.6); that is not explained, and no rule is made of it.  Bound
+// by HBM: 8192 tokens of 4096 in bf16 with a copy of the result for every rank (1.2 GB) 205 us, 5.9 TB/s.  A grid that stays
+// and keeps its weights in registers took 240 where this took 228.
 struct NormArgs {
     const char* partials[SAR_MAX_RANKS];
     const char* residual;
@@ -813,7 +815,10 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
     const uint32_t many = blockDim.x / b.row_threads, mine = many == 1 ? 0u : uniform(threadIdx.x / b.row_threads);
     const RowPart r{threadIdx.x - mine * b.row_threads, b.row_threads};
     RowSum sum{scratch, 0u, b.row_threads / kWave, uniform(threadIdx.x / kWave), threadIdx.x & (kWave - 1)};
-    // 16 elements a thread: two of the three column sums (128 KB) stay in LDS, or 48 registers more would be spilled
+    // 16 elements a thread: two of the three column sums (128 KB) stay in LDS (206 -> 131 us for 1000 tokens of 16384).  The
+    // compiler spills even so, 76 registers in bf16, 49 in f16 and 64 in f32 (228, 200 and 260 bytes a lane): from and to
+    // four ranks those 1000 tokens in bf16 take 161 us for 476 MB of their own and some 300 MB of scratch.  Eight elements: 5 in
+    // bf16 and 2 in f16, f32 none.
     constexpr bool kInLds = V * VE > 8;
     __shared__ f4 lds[kInLds ? 2 * (V * VE / 4) * kNormThreads : 1];
     Columns<V, VE, kInLds> col_pre, col_post;
@@ -897,7 +902,7 @@ __global__ __launch_bounds__(kNormThreads) void reduce_norm_backward_kernel(cons
             store_row<DT, VE, V, NT>(b.grad_residual + at, 0, 1, h, a, r);
         }
         float gate_dot = 0.f;
-        if (kInLds) load_gates();                      // again, from the cache: kept they would be spilled
+        if (kInLds) load_gates();                      // again, from the cache: kept they would be spilled too
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const Place<DT, VE> p(r.at + v * r.step, a.nvec, a.dim);
@@ -1125,7 +1130,7 @@ template <int DT> void launch_combine(hipStream_t st, const MoveArgs& a) {
 
 // A wave takes a token, with as many vectors a lane as the row has; four waves share one where the row is longer than
 // that, or where there are too few tokens to keep the chip busy (32 tokens of 2048, eight choices: 5.4 us shared, 7.3 not;
-// 4099 of 1001, two choices: 13.3 shared, 11.7 not).  Two rows at a time: four cost registers and with them waves (50000
+// 4099 of 1001, two choices: 13.3 shared, 11.7 not; nothing in between was measured).  Two rows at a time: four cost registers and with them waves (50000
 // tokens of 256, one choice: 36.7 us against 46.1).
 template <int DT> void launch_combine_backward(hipStream_t st, const MoveArgs& a) {
     const bool shared = a.nvec > 4 * kWave || (a.nvec > kWave && a.tokens < 2048);
