@@ -30,18 +30,25 @@ class Routing:
     slot's row among the rows sorted by expert, -1 = dropped.  ``slot_of_row`` [tokens * topk]: the slot (token * topk
     + choice) of each row, -1 behind the last.  ``offsets`` [num_experts + 1]: first row of each expert, then the
     number of rows; ``rank_offsets`` [ranks + 1]: the same for the ranks that own the experts.  All int32 on the GPU.  The tensors
-    stay as they are until the backward pass of every call that took them has run; autograd raises if they did not."""
+    stay as they are until the backward pass of every call that took them has run; autograd raises if they did not.
+    A routing put together by hand is checked here, once, so its parts cannot be exchanged afterwards; row numbers outside
+    the rows count as dropped, and rows below ``offsets[-1]`` that no slot names are left unwritten by ``dispatch``."""
 
     __slots__ = ("row_of_slot", "slot_of_row", "offsets", "num_experts", "ranks")
 
     def __init__(self, row_of_slot, slot_of_row, offsets, num_experts: int, ranks: int):
-        if row_of_slot.dim() != 2 or slot_of_row.numel() != row_of_slot.numel() or offsets.numel() != num_experts + 1 or num_experts % ranks:
+        if ranks < 1 or num_experts < 1 or row_of_slot.dim() != 2 or slot_of_row.numel() != row_of_slot.numel() or offsets.numel() != num_experts + 1 or num_experts % ranks:
             raise ValueError("row_of_slot [tokens, topk], slot_of_row [tokens * topk] and offsets [num_experts + 1] do not fit each other")
         for t in (row_of_slot, slot_of_row, offsets):
             if t.dtype is not torch.int32 or not t.is_contiguous() or t.device != offsets.device:
                 raise ValueError("a routing is made of contiguous int32 tensors on one device")
-        self.row_of_slot, self.slot_of_row, self.offsets = row_of_slot, slot_of_row, offsets
-        self.num_experts, self.ranks = num_experts, ranks
+        _fill(self, row_of_slot, slot_of_row, offsets, num_experts, ranks)
+
+    def __setattr__(self, name, value):
+        raise AttributeError("the parts of a routing are checked when it is made: make another Routing")
+
+    def __reduce__(self):
+        return Routing, (self.row_of_slot, self.slot_of_row, self.offsets, self.num_experts, self.ranks)
 
     @property
     def tokens(self) -> int:
@@ -54,6 +61,15 @@ class Routing:
     @property
     def rank_offsets(self):
         return self.offsets[::self.num_experts // self.ranks]
+
+
+_PARTS = tuple(getattr(Routing, name).__set__ for name in Routing.__slots__)
+
+
+def _fill(routing: Routing, *parts) -> Routing:
+    for put, part in zip(_PARTS, parts):
+        put(routing, part)
+    return routing
 
 
 class ReduceNormSaved(NamedTuple):
@@ -206,7 +222,7 @@ def route(group, experts, num_experts: int) -> Routing:
     work = torch.empty(need // 4, dtype=torch.int32, device=device) if need else None
     lib.check(lib.lib.sar_route(group.device, _raw_stream(group.device), experts.data_ptr(), experts.element_size(), tokens, topk, num_experts,
                                 row_of_slot.data_ptr(), slot_of_row.data_ptr(), offsets.data_ptr(), _ptr(work), need))
-    return Routing(row_of_slot, slot_of_row, offsets, num_experts, group.n)
+    return _fill(object.__new__(Routing), row_of_slot, slot_of_row, offsets, num_experts, group.n)
 
 
 # ---- dispatch, combine -----------------------------------------------------------------------------------------

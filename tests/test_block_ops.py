@@ -456,3 +456,21 @@ def test_the_capture_check_asks_the_tensors_own_device(monkeypatch):
     assert block_ops._recording(Leaf(0)) and now == [0]
     now[0] = 1
     assert block_ops._recording(Leaf(0)) and now == [1]
+
+
+def test_the_parts_of_a_routing_stay(recorder):
+    """They are checked when a routing is made and believed afterwards."""
+    import copy
+    import pickle
+    r = routing()
+    for name, value in [("row_of_slot", torch.zeros(2, 3, dtype=torch.int32).t()), ("row_of_slot", r.row_of_slot.long()), ("offsets", r.offsets[:3]),
+                        ("num_experts", 1 << 20), ("ranks", 0)]:
+        with pytest.raises(AttributeError, match="make another"):
+            setattr(r, name, value)
+    for again in (copy.copy(r), copy.deepcopy(r), pickle.loads(pickle.dumps(r)), recorder.route(torch.zeros(3, 2, dtype=torch.int64), 8)):
+        assert isinstance(again, block_ops.Routing) and again.row_of_slot.shape == (3, 2) and (again.num_experts, again.ranks, again.tokens) == (8, 4, 3)
+        assert again.rank_offsets.shape == (5,)
+    i = lambda *shape: torch.zeros(*shape, dtype=torch.int32)
+    for experts, ranks in [(8, 0), (8, -4), (0, 4)]:
+        with pytest.raises(ValueError):
+            block_ops.Routing(i(3, 2), i(6), i(experts + 1), experts, ranks)
