@@ -135,10 +135,9 @@ def _refuse_tracers():
 
 
 def _refuse_recorders():
-    inner = _transforms()
     if (_tracing() or any(m.is_infra_mode() for m in torch.utils._python_dispatch._get_current_dispatch_mode_stack())
             or torch._C._dispatch_tls_is_dispatch_key_included(torch._C.DispatchKey.PreDispatch)
-            or (inner is not None and inner.key() == torch._C._functorch.TransformType.Functionalize)):
+            or any(i.key() == torch._C._functorch.TransformType.Functionalize for i in torch._C._functorch.get_interpreter_stack() or ())):
         raise RuntimeError("the block operators cannot be traced: their kernels are no torch operations")
 
 

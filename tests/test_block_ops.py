@@ -312,7 +312,8 @@ def test_tracers_are_refused(recorder):
         return f
     for name, call in calls:
         for how in (lambda f: make_fx(f)(x), lambda f: make_fx(f, pre_dispatch=True)(x), lambda f: make_fx(f, tracing_mode="symbolic")(x),
-                    lambda f: torch.jit.trace(f, x, check_trace=False), lambda f: torch.func.functionalize(f)(x)):
+                    lambda f: torch.jit.trace(f, x, check_trace=False), lambda f: torch.func.functionalize(f)(x),
+                    lambda f: torch.func.functionalize(torch.vmap(f))(x)):
             with pytest.raises(RuntimeError, match="cannot be traced"):
                 how(also(call))
                 pytest.fail(name)
