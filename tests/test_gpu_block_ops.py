@@ -945,3 +945,103 @@ def test_streaming_norms(groups, dtype, dim, n, partials, gather, gate):
                 check(back.gate[part], want["gate"], a)
     for k, (v, e) in sums.items():
         check(getattr(back, k), B(v, 1.25 * e), k)
+
+
+# ---- inside other parts of torch ------------------------------------------------------------------------------------
+
+def small_block(g, r):
+    def f(x, w, v):
+        y = g.combine(torch.tanh(g.dispatch(x * 2, r)), r, w)
+        hidden, normed = g.reduce_norm([y, x, y, x], x, pre_weight=v, post_weight=v, gate=v, gather=False)
+        return hidden + normed
+    return f
+
+
+def small_inputs():
+    return (randn(2, 60, 72).requires_grad_(True), torch.softmax(randn(3, 60, 2), 1).requires_grad_(True),
+            randn(4, 72, mean=1.0, scale=0.1).requires_grad_(True))
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_under_activation_checkpointing(groups, reentrant):
+    from torch.utils.checkpoint import checkpoint
+    g = groups(4)
+    f, leaves = small_block(g, g.route(choices(1, 60, 2, 8, 0.2), 8)), small_inputs()
+    for t in leaves:
+        t.grad = None
+    f(*leaves).square().sum().backward()
+    want = [t.grad.clone() for t in leaves]
+    for t in leaves:
+        t.grad = None
+    checkpoint(f, *leaves, use_reentrant=reentrant).square().sum().backward()
+    assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+
+
+def test_under_torch_compile(groups):
+    """The graph breaks at the calls, which run as they are (no code is generated: the eager backend)."""
+    g = groups(4)
+    f, leaves = small_block(g, g.route(choices(1, 60, 2, 8, 0.2), 8)), small_inputs()
+    out, got = f(*leaves), torch.compile(f, backend="eager")(*leaves)
+    assert torch.equal(out, got)
+    for a, b in zip(torch.autograd.grad(out.sum(), leaves), torch.autograd.grad(got.sum(), leaves)):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        assert torch.equal(torch.compile(f, backend="eager")(*leaves), out)
+
+
+def test_two_threads_at_once(groups):
+    """Each on a stream of its own."""
+    import threading
+    g, want, got, went_wrong = groups(4), {}, {}, []
+    jobs = {i: (choices(i, 500 + 300 * i, 3, 8, 0.1), randn(i, 500 + 300 * i, 136)) for i in range(2)}
+
+    def work(e, x):
+        r = g.route(e, 8)
+        return g.reduce_norm(g.combine(g.dispatch(x, r), r), x, pre_weight=x[0].contiguous(), gather=False)
+    for i, job in jobs.items():
+        want[i] = work(*job)
+    torch.cuda.synchronize()
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[i] = [work(*jobs[i]) for _ in range(30)]
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:          # noqa: BLE001 (told to the test's own thread)
+            went_wrong.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not went_wrong, went_wrong
+    for i in jobs:
+        assert all(torch.equal(a, b) for run_ in got[i] for a, b in zip(run_, want[i])), i
+
+
+def test_the_most_slots_there_are(groups):
+    """2^31 - 1 of them: expert 3 i mod 8 for slot i, so its row is the expert's first plus i / 8.  One element a row."""
+    g, n, step = groups(4), 2 ** 31 - 1, 1 << 26
+    ids = torch.empty(n, 1, dtype=torch.int32, device="cuda")
+    x = torch.empty(n, 1, dtype=torch.float16, device="cuda")
+    for a in range(0, n, step):
+        i = torch.arange(a, min(n, a + step), device="cuda")
+        ids[a:a + step, 0] = (3 * i % 8).int()
+        x[a:a + step, 0] = (i % 2039).half()
+    r = g.route(ids, 8)
+    counts = [(n - first + 7) // 8 for first in range(8)]                     # of slots i = first mod 8
+    per_expert = {3 * first % 8: c for first, c in enumerate(counts)}
+    starts = np.concatenate([[0], np.cumsum([per_expert[e] for e in range(8)])])
+    assert np.array_equal(r.offsets.cpu().numpy(), starts)
+    first = torch.from_numpy(starts).cuda()
+    rows = g.dispatch(x, r)
+    for a in range(0, n, step):
+        i = torch.arange(a, min(n, a + step), device="cuda")
+        row = first[3 * i % 8] + i // 8
+        assert torch.equal(r.row_of_slot[a:a + step, 0].long(), row), a
+        assert torch.equal(r.slot_of_row[row].long(), i), a
+        assert torch.equal(rows[row, 0], x[a:a + step, 0]), a
+    del ids
+    assert torch.equal(g.combine(rows, r), x)
+    with pytest.raises(ValueError, match="2\\^31"):
+        g.route(torch.empty(2 ** 30, 2, dtype=torch.int32, device="cuda"), 8)
