@@ -505,10 +505,10 @@ uint64_t sar_route_workspace(int64_t tokens, int topk, int num_experts);
 int sar_route(int device, void* stream, const void* experts, int index_bytes, int64_t tokens, int topk, int num_experts,
               int32_t* row_of_slot, int32_t* slot_of_row, int32_t* offsets, void* workspace, uint64_t workspace_bytes);
 
-/* rows[row_of_slot[t][k]][:] = tokens[t][:], and zeros in the rows behind offsets[num_experts].  With weights
- * (elements of weight_dtype, NULL = none) rows are weights[t][k] * tokens[t][:], rounded once.  rows has
- * tokens * topk rows of `dim` elements of dtype.  The gradient of sar_combine without a gradient of its weights, and,
- * without weights, the way to the experts. */
+/* rows[row_of_slot[t][k]][:] = tokens[t][:], and zeros in the rows behind offsets[num_experts] (rows in front of it that
+ * no slot names, which sar_route never leaves, stay as they were).  With weights (elements of weight_dtype, NULL = none)
+ * rows are weights[t][k] * tokens[t][:], rounded once.  rows has tokens * topk rows of `dim` elements of dtype.  The
+ * gradient of sar_combine without a gradient of its weights, and, without weights, the way to the experts. */
 int sar_dispatch(int device, void* stream, int dtype, const void* token_rows, int64_t tokens, int topk, int64_t dim,
                  const int32_t* row_of_slot, const int32_t* offsets, int num_experts, const void* weights, int weight_dtype,
                  void* rows);

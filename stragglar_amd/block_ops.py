@@ -48,7 +48,7 @@ class Routing:
         raise AttributeError("the parts of a routing are checked when it is made: make another Routing")
 
     def __reduce__(self):
-        return Routing, (self.row_of_slot, self.slot_of_row, self.offsets, self.num_experts, self.ranks)
+        return type(self), (self.row_of_slot, self.slot_of_row, self.offsets, self.num_experts, self.ranks)
 
     @property
     def tokens(self) -> int:
@@ -281,7 +281,7 @@ class _Dispatch(_Node):
     @staticmethod
     def forward(ctx, rows, plain):
         group, routing = plain
-        ctx.plain = (group, routing.row_of_slot.shape, _hooks(True))
+        ctx.plain = (group, routing.row_of_slot.shape, _hooks(True) is not None)
         ctx.save_for_backward(_savable(routing.row_of_slot))
         return _dispatch(group, rows, routing.row_of_slot, routing.offsets)
 
