@@ -1390,6 +1390,8 @@ int sar_reduce_norm_backward(int device, void* stream, const sar_reduce_norm_arg
         if (g->grad_pre_weight && !forward->pre_weight) return refuse("grad_pre_weight without pre_weight");
         if (g->grad_post_weight && !forward->post_weight) return refuse("grad_post_weight without post_weight");
         if (g->grad_gate && forward->gate_kind == SAR_GATE_NONE) return refuse("grad_gate without a gate");
+        // with no tokens the kernel still runs, for the weights' zero gradients, and holds a channel gate in registers
+        if (channel && !forward->gate) return refuse("gate is null");
         if (g->total_dtype != SAR_F32 && g->total_dtype != forward->dtype) return refuse("total must be of dtype or 32-bit floats");
         if (forward->tokens && (!g->total || !forward->stats)) return refuse("total or stats is null");
         if (!aligned(g->total, elem_size(g->total_dtype)) || !aligned(forward->stats, 4) || !aligned(g->grad_hidden, es) || !aligned(g->grad_normed, es) ||

@@ -475,3 +475,11 @@ def test_the_parts_of_a_routing_stay(recorder):
     for experts, ranks in [(8, 0), (8, -4), (0, 4)]:
         with pytest.raises(ValueError):
             block_ops.Routing(i(3, 2), i(6), i(experts + 1), experts, ranks)
+
+
+def test_the_backward_pass_of_no_tokens_wants_its_channel_gate(sarlib):
+    """The kernel runs even then and reads the gate's `dim` elements: a null pointer has to end on the host."""
+    p = 0x10000
+    a = capi.ReduceNormArgs(dtype=0, sources=1, copies=1, tokens=0, dim=8, eps=1e-6, residual_scale=1.0, gate_kind=1, post_weight=p)
+    g = capi.ReduceNormGrads(total_dtype=0, grad_post_weight=p)
+    refused(sarlib, sarlib.lib.sar_reduce_norm_backward(0, None, ctypes.byref(a), ctypes.byref(g)), "gate is null")
